@@ -509,6 +509,81 @@ LCU_API int lcu_op_sample_rows(lcu_kv_pair *out, lcu_kv_pair *out_copy, const vo
  * stream need no clearing.  Same result as lcu_op_sample_rows with args_dev == NULL. */
 LCU_API int lcu_argmax_rows_noalloc(lcu_kv_pair *out, const void *logits, int rows, size_t n, int dt, lcu_stream_t s);
 
+/* ------------------------------------------------------------------ operators on a caller's pages, and of drafted tokens
+ * For hosts that run a round's operators themselves: a round of drafted tokens or of many samples of one prompt is lcu_op_kv_append,
+ * lcu_op_attention_prefix, the projections, lcu_op_softmax_rows, lcu_op_verify_drafts.  (No counterparts in the reference: one
+ * contiguous cache per session, exec/kv_cache.rs:15-54; one sampled token per row, exec/output_head.rs:104-113.)  As for every
+ * lcu_op_*: no allocation, no synchronisation, the stream's device is current; two calls in flight at once share no output and no workspace.
+ * Indices that live on the device are checked there: what each call does with one that is out of range stands with the call. */
+
+/* Pages of one layer: the row of token slot t (0 <= t < page_tokens) and KV head h of page p starts at k (or v) + p * stride_page +
+ * t * stride_tok + h * stride_head.  lcu_kv_layer_pages fills it for a context's own pool. */
+typedef struct {
+    void *k, *v;
+    int64_t stride_page;  /* elements */
+    int32_t stride_tok, stride_head;
+    int32_t n_pages;      /* ids outside [0, n_pages) name no page */
+    int32_t page_tokens;  /* power of two in [8,128] */
+} lcu_kv_pages;
+/* What is done to rows of queries and keys: y = x w / sqrt(mean(x^2) + eps) per head (where there are weights), then the first
+ * rot_dims values of a head are rotated by their token's position.  32-bit arithmetic, one rounding. */
+typedef struct {
+    const void *q_norm, *k_norm;  /* [dh] weights of the queries' and the keys' norm; NULL: no norm */
+    const float *sin_t, *cos_t;   /* [n_pos, rot_dims / 2]; may be NULL when rot_dims == 0 */
+    int32_t norm_dt;              /* of the weights: the rows' dtype or LCU_F32 */
+    float eps;
+    int32_t n_pos;
+    int32_t rot_dims;             /* even, 0 .. dh */
+    int32_t rot_halves;           /* 0: pairs (2 i, 2 i + 1) as in lcu_op_rope; 1: pairs (i, i + rot_dims / 2) */
+} lcu_qk_prep;
+/* The pages of `layer` of a context's pool (contexts of lcu_ctx_create), and the ids of a sequence's pages in order (host memory; up to
+ * cap of them are written, *n_out is how many there are). */
+LCU_API int lcu_kv_layer_pages(const lcu_ctx *ctx, int layer, lcu_kv_pages *out);
+LCU_API int lcu_seq_pages(const lcu_ctx *ctx, int seq, int32_t *ids, int cap, int *n_out);
+/* Queries [n, nh, dh] and keys [n, nkvh, dh] in one pass (nh or nkvh may be 0), dh <= 256, dt LCU_F16, LCU_BF16 or LCU_F32.  Outputs may be
+ * the inputs (same strides), and may not overlap them otherwise.  A token whose position is not below n_pos is left unwritten. */
+LCU_API int lcu_op_qk_norm_rope(void *q_out, int stride_tok_qo, int stride_head_qo, const void *q, int stride_tok_q, int stride_head_q, void *k_out,
+                                int stride_tok_ko, int stride_head_ko, const void *k, int stride_tok_k, int stride_head_k, const uint32_t *pos,
+                                const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s);
+/* Keys and values [n, nkvh, dh] of n tokens into pages, keys (and queries [n, nh, dh], into q_out; nh may be 0) as lcu_op_qk_norm_rope
+ * does it on the way; prep NULL: keys go in as they are, nh is 0, pos is not read.  Token t belongs to sequence tok_seq[t], whose pages are
+ * table[tok_seq[t] * table_stride ..], and goes to slot[t] of it (its place in those pages; pos[t] is what it is rotated by).  tables, tok_seq,
+ * slot and pos on the device.  Nothing is written of a token with tok_seq outside [0, n_seq) (a padded round), a slot behind the
+ * table, a page id that names no page, or a position not below n_pos.  No two tokens of a call may have the same place (what it
+ * then holds is either's, in pieces). */
+LCU_API int lcu_op_kv_append(const lcu_kv_pages *pages, const int32_t *table, int table_stride, int n_seq, const int32_t *tok_seq, const uint32_t *slot,
+                             const void *k, int stride_tok_k, int stride_head_k, const void *v, int stride_tok_v, int stride_head_v, void *q_out,
+                             int stride_tok_qo, int stride_head_qo, const void *q, int stride_tok_q, int stride_head_q, const uint32_t *pos,
+                             const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s);
+/* Attention of n tokens whose sequences begin with the same prefix: token t sees the first prefix_len slots of the pages prefix_table and
+ * the first tok_ctx[t] slots of its sequence's own pages (table, as above; positions of the prefix are not repeated there).  o, q
+ * [n, nh, dh]; query head h reads KV head h / (nh / nkvh); scores are scaled by `scale` > 0.  dh 64 or 128, nh / nkvh up to 16, dt LCU_F16 or LCU_BF16.
+ * The prefix is read once for all tokens.  f32 scores and softmax, weights rounded to dt ahead of the product with the values, one rounding
+ * of the output.  Rows of q, o and the pages start on 16 bytes.  Tokens with tok_seq outside [0, n_seq) are left unwritten; tok_ctx counts at
+ * most table_stride pages; positions on page ids that name no page are not seen; a token that sees nothing gets zeros.
+ * table may be NULL with table_stride 0: no sequence has pages of its own.  Workspace: lcu_attention_prefix_workspace_size bytes, 256-byte
+ * aligned, contents irrelevant (0 bytes: NULL will do). */
+LCU_API size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len);
+LCU_API int lcu_op_attention_prefix(void *o, int stride_tok_o, int stride_head_o, const void *q, int stride_tok_q, int stride_head_q,
+                                    const lcu_kv_pages *pages, const int32_t *prefix_table, uint32_t prefix_len, const int32_t *table,
+                                    int table_stride, int n_seq, const int32_t *tok_seq, const uint32_t *tok_ctx, int n, int nh, int nkvh, int dh,
+                                    float scale, int dt, void *workspace, size_t workspace_len, lcu_stream_t s);
+/* probs[r, j] = exp((x_j - max) / T) / sum over the n logits of row r, f32; T = temperature[r] (device, >= 0; NULL: 1 everywhere).  T = 0: 1 at
+ * the lowest index of the largest logit, 0 elsewhere.  Logits of dtype dt (F16, BF16, F32); strides from row to row in elements.
+ * Logits of -inf get 0; a row of nothing else gets zeros; with T > 0 a row that holds NaN or +inf is NaN, with T = 0 NaN never is the largest. */
+LCU_API int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *logits, size_t stride_l, const float *temperature, int rows, size_t n, int dt,
+                                lcu_stream_t s);
+/* Verification of drafted tokens (speculative sampling) from given random numbers.  Sequence b brings n_drafted[b] <= k drafts (NULL: k
+ * each; counts are clamped to [0, k]); its target probabilities are the rows b (k + 1) + i, those that the drafts were drawn from the rows
+ * b k + i (NULL: each draft is certain, probability 1 at its token), probabilities of dtype dt (F16, BF16, F32) and strides in elements.
+ * Draft i, drafted[b k + i], is accepted while randoms[b (k + 1) + i] * q(draft) < p(draft).  Behind the accepted ones comes one more token, the
+ * first whose running sum of weights exceeds randoms[b (k + 1) + k] times their total: weights max(p - q, 0) at a rejected draft (p where
+ * these are all zero), p behind the last draft.  64-bit comparisons and sums; weights that are no positive finite number count as 0, and a draft outside
+ * the vocabulary is rejected.  accepted[b]: drafts accepted; tokens[b (k + 1) ..]: these, the token behind them (-1 where no
+ * weight is positive), then -1.  Random numbers in [0,1). */
+LCU_API int lcu_op_verify_drafts(int32_t *accepted, int32_t *tokens, const void *target, size_t stride_t, const void *draft, size_t stride_d,
+                                 const int32_t *drafted, const int32_t *n_drafted, const float *randoms, int n_seq, int k, size_t n, int dt, lcu_stream_t s);
+
 /* ------------------------------------------------------------------ collectives set-up
  * Thin wrappers over the NCCL library found at run time == `CommunicatorGroup::new`
  * (exec/engine.rs:86), one process per GPU instead of one thread per GPU. */

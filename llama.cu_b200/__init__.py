@@ -82,6 +82,18 @@ class Req(C.Structure):
     _fields_ = [("seq", C.c_int32), ("pos", C.c_uint32), ("len", C.c_uint32)]
 
 
+class KvPages(C.Structure):
+    """Pages of one layer as the stand-alone operators take them (lcu_kv_pages)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("stride_page", C.c_int64)] + [
+        (n, C.c_int32) for n in ("stride_tok", "stride_head", "n_pages", "page_tokens")]
+
+
+class QkPrep(C.Structure):
+    """Norm and rotation of queries and keys (lcu_qk_prep)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q_norm", "k_norm", "sin_t", "cos_t")] + [
+        ("norm_dt", C.c_int32), ("eps", C.c_float)] + [(n, C.c_int32) for n in ("n_pos", "rot_dims", "rot_halves")]
+
+
 class RoundInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_tok", "n_req", "n_fast", "n_finished", "n_overflow")]
 
@@ -189,6 +201,18 @@ _SIGNATURES = {
     "lcu_op_sample_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p,
                                      C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "lcu_argmax_rows_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_void_p]),
+    "lcu_kv_layer_pages": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(KvPages)]),
+    "lcu_seq_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_int)]),
+    "lcu_op_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_int, C.c_int] * 4 + [C.c_void_p, C.POINTER(QkPrep)] + [C.c_int] * 5 + [C.c_void_p]),
+    "lcu_op_kv_append": (C.c_int, [C.POINTER(KvPages), C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p] + [C.c_void_p, C.c_int, C.c_int] * 4 +
+                         [C.c_void_p, C.POINTER(QkPrep)] + [C.c_int] * 5 + [C.c_void_p]),
+    "lcu_attention_prefix_workspace_size": (C.c_size_t, [C.c_int] * 4 + [C.c_uint32]),
+    "lcu_op_attention_prefix": (C.c_int, [C.c_void_p, C.c_int, C.c_int] * 2 + [C.POINTER(KvPages), C.c_void_p, C.c_uint32, C.c_void_p, C.c_int, C.c_int,
+                                                                               C.c_void_p, C.c_void_p] + [C.c_int] * 4 +
+                                [C.c_float, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "lcu_op_softmax_rows": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_void_p]),
+    "lcu_op_verify_drafts": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                       C.c_int, C.c_size_t, C.c_int, C.c_void_p]),
     "lcu_comm_unique_id": (C.c_int, [C.c_void_p]),
     "lcu_comm_init_rank": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
     "lcu_comm_destroy": (C.c_int, [C.c_void_p]),
@@ -361,6 +385,20 @@ class Context:
     def seq_resumable(self, seq, length):
         """Largest position <= length the sequence can be continued from (recurrent state cannot be rolled back)."""
         return self.lib.lcu_seq_resumable(self.h, seq, length)
+
+    def seq_pages(self, seq):
+        """Ids of the sequence's pages in order."""
+        n = C.c_int()
+        check(self.lib.lcu_seq_pages(self.h, seq, None, 0, C.byref(n)))
+        ids = np.empty(n.value, np.int32)
+        check(self.lib.lcu_seq_pages(self.h, seq, ids.ctypes.data, n.value, C.byref(n)))
+        return ids
+
+    def layer_pages(self, layer):
+        """The pool's pages of one layer, as lcu_op_kv_append and lcu_op_attention_prefix take them."""
+        pages = KvPages()
+        check(self.lib.lcu_kv_layer_pages(self.h, layer, C.byref(pages)))
+        return pages
 
     def seq_free(self, seq):
         check(self.lib.lcu_seq_free(self.h, seq))

@@ -533,6 +533,32 @@ int lcu_seq_len(const lcu_ctx *c, int seq) {
     return (int)c->seqs[seq].len;
 }
 
+int lcu_seq_pages(const lcu_ctx *c, int seq, int32_t *ids, int cap, int *n_out) {
+    LCU_REQUIRE(c && n_out && seq >= 0 && seq < (int)c->seqs.size() && c->seqs[seq].used, "seq_pages: bad sequence %d", seq);
+    LCU_REQUIRE(cap >= 0 && (cap == 0 || ids), "seq_pages: no room for %d ids", cap);
+    const auto &pages = c->seqs[seq].pages;
+    *n_out = (int)pages.size();
+    for (int i = 0; i < cap && i < *n_out; ++i) ids[i] = pages[i];
+    return LCU_OK;
+}
+
+int lcu_kv_layer_pages(const lcu_ctx *c, int layer, lcu_kv_pages *out) {
+    LCU_REQUIRE(c && out, "kv_layer_pages: null argument");
+    LCU_REQUIRE(!c->stack, "kv_layer_pages: the layers of this context have caches of their own forms");
+    LCU_REQUIRE(c->pool, "kv_layer_pages: no pool yet");
+    LCU_REQUIRE(layer >= 0 && layer < c->geom.n_layers, "kv_layer_pages: layer %d of %d", layer, c->geom.n_layers);
+    unsigned char *pool = reinterpret_cast<unsigned char *>(c->pool);
+    const size_t es = dt_bytes(c->dt);
+    out->k = pool + c->geom.block_off(0, layer, 0, 0) * es;
+    out->v = pool + c->geom.block_off(0, layer, 1, 0) * es;
+    out->stride_page = (int64_t)c->geom.page_elems;
+    out->stride_tok = c->geom.dh;
+    out->stride_head = c->geom.page_tokens * c->geom.dh;
+    out->n_pages = c->n_pages;
+    out->page_tokens = c->geom.page_tokens;
+    return LCU_OK;
+}
+
 int lcu_seq_free(lcu_ctx *c, int seq) {
     LCU_REQUIRE(c && seq >= 0 && seq < (int)c->seqs.size() && c->seqs[seq].used, "seq_free: bad sequence %d", seq);
     SeqState &s = c->seqs[seq];

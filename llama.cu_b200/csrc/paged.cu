@@ -1,0 +1,329 @@
+// Queries and keys of a round, normed per head and rotated in one pass, and the appending of keys and values to a paged cache on the way
+// (no counterpart in the reference, which norms no heads and whose cache is one stretch per session, exec/kv_cache.rs:15-54).
+//
+//   y = x w / sqrt(mean(x^2) + eps)                   per head, where there are weights
+//   (a, b) -> (a cos - b sin, a sin + b cos)          of the first rot_dims values, pairs (2 i, 2 i + 1) or (i, i + rot_dims / 2)
+//
+// all in 32 bits with one rounding at the end.  Bound by HBM: every row is read once and written once.  A row of dh values is held by
+// dh / 8 lanes, 8 values each (the partner of a half-split pair is a shuffle away), and a thread keeps the sin and cos of its values
+// for every row of the token that it takes: a block is a token, so the tables are read once per thread and not once per row.
+#include "paged.cuh"
+
+namespace lcu {
+
+constexpr int RW_THREADS = 256;
+constexpr int RW_MAX_HEAD = 256;
+
+struct RowsArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_out;              // k_out: rows of lcu_op_qk_norm_rope, null when keys go to pages
+    int stq, shq, stk, shk, stv, shv, stqo, shqo, stko, shko;
+    lcu_kv_pages pages;
+    const int32_t *table, *tok_seq;
+    const uint32_t *slot, *pos;
+    int table_stride, n_seq, page_shift;
+    const void *q_w, *k_w;
+    const float *sin_t, *cos_t;
+    float eps;
+    uint32_t n_pos;
+    int w_f32, rot, halves, nh, nkvh, n_v, dh;  // n_v: value rows of a token (0 without a cache)
+};
+
+// Where a token goes: false when nothing of it is written (padding, or indices outside what the call names).
+__device__ __forceinline__ bool rw_place(const RowsArgs &a, int t, uint32_t &p, size_t &off) {
+    p = a.pos && a.rot ? a.pos[t] : 0u;
+    if (a.rot && p >= a.n_pos) return false;
+    off = 0;
+    if (!a.table) return true;
+    const int seq = a.tok_seq[t];
+    const uint32_t slot = a.slot[t];
+    if (seq < 0 || seq >= a.n_seq || (slot >> a.page_shift) >= (uint32_t)a.table_stride) return false;
+    const int page = a.table[(size_t)seq * a.table_stride + (slot >> a.page_shift)];
+    if (page < 0 || page >= a.pages.n_pages) return false;
+    off = (size_t)page * a.pages.stride_page + (size_t)(slot & ((1u << a.page_shift) - 1)) * a.pages.stride_tok;
+    return true;
+}
+
+// row r of token t: queries, then keys, then values
+template <class T> __device__ __forceinline__ const T *rw_src(const RowsArgs &a, int t, int r) {
+    if (r < a.nh) return reinterpret_cast<const T *>(a.q) + (size_t)t * a.stq + (size_t)r * a.shq;
+    r -= a.nh;
+    if (r < a.nkvh) return reinterpret_cast<const T *>(a.k) + (size_t)t * a.stk + (size_t)r * a.shk;
+    return reinterpret_cast<const T *>(a.v) + (size_t)t * a.stv + (size_t)(r - a.nkvh) * a.shv;
+}
+template <class T> __device__ __forceinline__ T *rw_dst(const RowsArgs &a, int t, int r, size_t off) {
+    if (r < a.nh) return reinterpret_cast<T *>(a.q_out) + (size_t)t * a.stqo + (size_t)r * a.shqo;
+    r -= a.nh;
+    if (r < a.nkvh) {
+        if (!a.table) return reinterpret_cast<T *>(a.k_out) + (size_t)t * a.stko + (size_t)r * a.shko;
+        return reinterpret_cast<T *>(a.pages.k) + off + (size_t)r * a.pages.stride_head;
+    }
+    return reinterpret_cast<T *>(a.pages.v) + off + (size_t)(r - a.nkvh) * a.pages.stride_head;
+}
+
+// eight values of a row as 16-byte pieces
+template <class T> struct Row8 {
+    uint4 u;
+    __device__ __forceinline__ void load(const T *p) { u = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = u; }
+    __device__ __forceinline__ void get(float *f) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = Act<T>::to_f2(w[i]);
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void set(const float *f) {
+        u = make_uint4(Act<T>::pack(f[0], f[1]), Act<T>::pack(f[2], f[3]), Act<T>::pack(f[4], f[5]), Act<T>::pack(f[6], f[7]));
+    }
+};
+template <> struct Row8<float> {
+    float4 x, y;
+    __device__ __forceinline__ void load(const float *p) { x = reinterpret_cast<const float4 *>(p)[0]; y = reinterpret_cast<const float4 *>(p)[1]; }
+    __device__ __forceinline__ void store(float *p) const { reinterpret_cast<float4 *>(p)[0] = x; reinterpret_cast<float4 *>(p)[1] = y; }
+    __device__ __forceinline__ void get(float *f) const {
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+        f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+    }
+    __device__ __forceinline__ void set(const float *f) { x = make_float4(f[0], f[1], f[2], f[3]); y = make_float4(f[4], f[5], f[6], f[7]); }
+};
+
+template <class T> __device__ __forceinline__ float rw_f(T v) { return Act<T>::to_f(v); }
+template <> __device__ __forceinline__ float rw_f<float>(float v) { return v; }
+template <class T> __device__ __forceinline__ T rw_t(float v) { return Act<T>::from_f(v); }
+template <> __device__ __forceinline__ float rw_t<float>(float v) { return v; }
+
+// LPR lanes of a warp hold a row of dh <= 8 LPR values; R rows per lane group, requested before the first is used.
+template <class T, int LPR, int R>
+__global__ void __launch_bounds__(RW_THREADS) rows_kernel(const RowsArgs a) {
+    constexpr int GROUPS = RW_THREADS / LPR;
+    const int t = blockIdx.x, c = threadIdx.x % LPR, d = 8 * c, total = a.nh + a.nkvh + a.n_v;
+    const int r0 = blockIdx.y * (GROUPS * R) + threadIdx.x / LPR;
+    const bool in = d < a.dh;
+    Row8<T> x[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int r = r0 + j * GROUPS;
+        if (in && r < total) x[j].load(rw_src<T>(a, t, r) + d);
+    }
+    uint32_t p;
+    size_t off;
+    if (!rw_place(a, t, p, off)) return;
+    const int half = a.rot >> 1;
+    float sn[8], cs[8];  // of the 8 values (halves), or of the 4 pairs
+    const bool turned = d < a.rot;
+    if (turned) {
+        const size_t at = (size_t)p * half + (a.halves ? (d < half ? d : d - half) : d >> 1);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            if (i == 4 && !a.halves) break;
+            const float4 s4 = *reinterpret_cast<const float4 *>(a.sin_t + at + i), c4 = *reinterpret_cast<const float4 *>(a.cos_t + at + i);
+            sn[i] = s4.x; sn[i + 1] = s4.y; sn[i + 2] = s4.z; sn[i + 3] = s4.w;
+            cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
+        }
+    }
+    const int step = half >> 3, partner = a.halves && turned ? (d < half ? c + step : c - step) : c;  // lane of the row that holds the other halves
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int r = r0 + j * GROUPS;
+        const bool is_v = r >= a.nh + a.nkvh;  // (rows past the last take part in the shuffles)
+        const void *w = r < a.nh ? a.q_w : a.k_w;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 0.f;
+        if (in && r < total) x[j].get(f);
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w && !is_v && in) {
+            const float s = rsqrtf(ss / (float)a.dh + a.eps);
+            float g[8];
+            if (a.w_f32) {
+                Row8<float> u;
+                u.load(reinterpret_cast<const float *>(w) + d);
+                u.get(g);
+            } else {
+                Row8<T> u;
+                u.load(reinterpret_cast<const T *>(w) + d);
+                u.get(g);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * s * g[i];
+        }
+        if (a.halves) {
+            const float sgn = d < half ? -1.f : 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = __shfl_sync(0xffffffffu, f[i], partner, LPR);
+                if (turned && !is_v) f[i] = f[i] * cs[i] + sgn * y * sn[i];
+            }
+        } else if (turned && !is_v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = f[2 * i], v = f[2 * i + 1];
+                f[2 * i] = u * cs[i] - v * sn[i];
+                f[2 * i + 1] = u * sn[i] + v * cs[i];
+            }
+        }
+        if (!in || r >= total) continue;
+        if (!is_v) x[j].set(f);
+        x[j].store(rw_dst<T>(a, t, r, off) + d);
+    }
+}
+
+// Rows that are not in 16-byte pieces (sizes, strides or addresses that no multiple of 8 values allows): a warp per row, a value per
+// lane and step; the row passes through shared memory, so that it may be written where it was read.
+template <class T>
+__global__ void __launch_bounds__(RW_THREADS) rows_any_kernel(const RowsArgs a) {
+    __shared__ float rows[RW_THREADS / 32][RW_MAX_HEAD];
+    const int t = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * (RW_THREADS / 32) + (threadIdx.x >> 5);
+    uint32_t p;
+    size_t off;
+    if (r >= a.nh + a.nkvh + a.n_v || !rw_place(a, t, p, off)) return;
+    const T *src = rw_src<T>(a, t, r);
+    T *dst = rw_dst<T>(a, t, r, off);
+    if (r >= a.nh + a.nkvh) {
+        for (int i = lane; i < a.dh; i += 32) dst[i] = src[i];
+        return;
+    }
+    float *y = rows[threadIdx.x >> 5], ss = 0.f;
+    for (int i = lane; i < a.dh; i += 32) {
+        y[i] = rw_f<T>(src[i]);
+        ss = fmaf(y[i], y[i], ss);
+    }
+    if (const void *w = r < a.nh ? a.q_w : a.k_w) {
+        const float s = rsqrtf(warp_sum(ss) / (float)a.dh + a.eps);
+        for (int i = lane; i < a.dh; i += 32) y[i] = y[i] * s * (a.w_f32 ? reinterpret_cast<const float *>(w)[i] : rw_f<T>(reinterpret_cast<const T *>(w)[i]));
+    }
+    __syncwarp();
+    const int half = a.rot >> 1;
+    const float *sn = a.sin_t + (size_t)p * half, *cs = a.cos_t + (size_t)p * half;
+    for (int i = lane; i < a.dh; i += 32) {
+        float v = y[i];
+        if (i < a.rot) {
+            const bool first = a.halves ? i < half : (i & 1) == 0;
+            const int e = a.halves ? (first ? i + half : i - half) : i ^ 1, at = a.halves ? (first ? i : e) : i >> 1;
+            v = first ? v * cs[at] - y[e] * sn[at] : y[e] * sn[at] + v * cs[at];
+        }
+        dst[i] = rw_t<T>(v);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+template <class T, int LPR>
+static int rows_launch(const RowsArgs &a, int n, cudaStream_t s) {
+    constexpr int GROUPS = RW_THREADS / LPR;
+    const int rows = a.nh + a.nkvh + a.n_v, parts = (rows + GROUPS - 1) / GROUPS;
+    // few tokens: a block per pass over the heads (latency); many: a token's block keeps its tables for several passes
+    if ((long long)n * parts <= 8LL * sm_count() || parts == 1)
+        rows_kernel<T, LPR, 1><<<dim3(n, parts), RW_THREADS, 0, s>>>(a);
+    else
+        rows_kernel<T, LPR, 3><<<dim3(n, (parts + 2) / 3), RW_THREADS, 0, s>>>(a);
+    LCU_CHECK_CUDA(cudaGetLastError());
+    return LCU_OK;
+}
+
+template <class T>
+static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
+    if (!vec) {
+        const int rows = a.nh + a.nkvh + a.n_v, per = RW_THREADS / 32;
+        rows_any_kernel<T><<<dim3(n, (rows + per - 1) / per), RW_THREADS, 0, s>>>(a);
+        LCU_CHECK_CUDA(cudaGetLastError());
+        return LCU_OK;
+    }
+    const int lanes = a.dh / 8;
+    return lanes <= 4 ? rows_launch<T, 4>(a, n, s) : lanes <= 8 ? rows_launch<T, 8>(a, n, s) : lanes <= 16 ? rows_launch<T, 16>(a, n, s) : rows_launch<T, 32>(a, n, s);
+}
+
+static int rows_run(RowsArgs &a, const lcu_qk_prep *prep, int n, int dt, const char *who, cudaStream_t s) {
+    LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "%s: dtype %d unsupported", who, dt);
+    LCU_REQUIRE(n >= 0 && a.nh >= 0 && a.nkvh >= 0 && a.nh + a.nkvh > 0 && (long long)a.nh + 2LL * a.nkvh <= 65535, "%s: %d tokens, %d and %d heads", who, n, a.nh, a.nkvh);
+    LCU_REQUIRE(a.dh >= 1 && a.dh <= RW_MAX_HEAD, "%s: heads of %d values (1..%d)", who, a.dh, RW_MAX_HEAD);
+    const int es = dt == LCU_F32 ? 4 : 2, per = 16 / es;
+    bool vec = a.dh % 8 == 0;
+    auto pieces = [&](const void *p, int st, int sh) { vec = vec && (uintptr_t)p % 16 == 0 && st % per == 0 && sh % per == 0; };
+    if (a.nh) {
+        pieces(a.q, a.stq, a.shq);
+        pieces(a.q_out, a.stqo, a.shqo);
+    }
+    if (a.nkvh) {
+        pieces(a.k, a.stk, a.shk);
+        if (!a.table) pieces(a.k_out, a.stko, a.shko);
+    }
+    if (a.table) {
+        pieces(a.v, a.stv, a.shv);
+        pieces(a.pages.k, a.pages.stride_tok, a.pages.stride_head);
+        pieces(a.pages.v, 0, 0);
+        vec = vec && a.pages.stride_page % per == 0;
+    }
+    if (prep) {
+        LCU_REQUIRE(prep->rot_dims >= 0 && prep->rot_dims % 2 == 0 && prep->rot_dims <= a.dh, "%s: %d rotated dimensions of %d", who, prep->rot_dims, a.dh);
+        LCU_REQUIRE(prep->rot_dims == 0 || (prep->sin_t && prep->cos_t && prep->n_pos >= 1 && a.pos), "%s: a rotation needs positions and tables", who);
+        LCU_REQUIRE((!prep->q_norm && !prep->k_norm) || prep->norm_dt == dt || prep->norm_dt == LCU_F32, "%s: norm weights of dtype %d beside dtype %d", who, prep->norm_dt, dt);
+        LCU_REQUIRE(prep->eps >= 0.f, "%s: eps %g", who, (double)prep->eps);
+        a.q_w = prep->q_norm;
+        a.k_w = prep->k_norm;
+        a.w_f32 = prep->norm_dt == LCU_F32;
+        a.eps = prep->eps;
+        a.rot = prep->rot_dims;
+        a.halves = prep->rot_halves != 0;
+        a.sin_t = prep->sin_t;
+        a.cos_t = prep->cos_t;
+        a.n_pos = (uint32_t)prep->n_pos;
+        pieces(a.q_w, 0, 0);
+        pieces(a.k_w, 0, 0);
+        if (a.rot) {
+            pieces(a.sin_t, 0, 0);
+            pieces(a.cos_t, 0, 0);
+            vec = vec && a.rot % (a.halves ? 16 : 8) == 0;
+        }
+    }
+    if (n == 0) return LCU_OK;
+    if (dt == LCU_F16) return rows_t<__half>(a, n, vec, s);
+    if (dt == LCU_BF16) return rows_t<__nv_bfloat16>(a, n, vec, s);
+    return rows_t<float>(a, n, vec, s);
+}
+
+int kv_pages_check(const lcu_kv_pages *p, const char *who) {
+    LCU_REQUIRE(p && p->k && p->v && p->n_pages >= 1, "%s: no pages", who);
+    LCU_REQUIRE(p->page_tokens >= 8 && p->page_tokens <= 128 && (p->page_tokens & (p->page_tokens - 1)) == 0,
+                "%s: pages of %d tokens (a power of two in [8,128])", who, p->page_tokens);
+    LCU_REQUIRE(p->stride_page > 0 && p->stride_tok > 0 && p->stride_head >= 0, "%s: page strides", who);
+    return LCU_OK;
+}
+
+}  // namespace lcu
+
+using namespace lcu;
+
+extern "C" int lcu_op_qk_norm_rope(void *q_out, int stqo, int shqo, const void *q, int stq, int shq, void *k_out, int stko, int shko, const void *k, int stk,
+                                   int shk, const uint32_t *pos, const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s) {
+    LCU_REQUIRE(prep && (nh <= 0 || n <= 0 || (q_out && q)) && (nkvh <= 0 || n <= 0 || (k_out && k)), "qk_norm_rope: null argument");
+    RowsArgs a{};
+    a.q = q; a.stq = stq; a.shq = shq; a.q_out = q_out; a.stqo = stqo; a.shqo = shqo;
+    a.k = k; a.stk = stk; a.shk = shk; a.k_out = k_out; a.stko = stko; a.shko = shko;
+    a.pos = pos; a.nh = nh; a.nkvh = nkvh; a.dh = dh;
+    return rows_run(a, prep, n, dt, "qk_norm_rope", as_stream(s));
+}
+
+extern "C" int lcu_op_kv_append(const lcu_kv_pages *pages, const int32_t *table, int table_stride, int n_seq, const int32_t *tok_seq, const uint32_t *slot,
+                                const void *k, int stk, int shk, const void *v, int stv, int shv, void *q_out, int stqo, int shqo, const void *q, int stq,
+                                int shq, const uint32_t *pos, const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s) {
+    int rc = kv_pages_check(pages, "kv_append");
+    if (rc) return rc;
+    LCU_REQUIRE(n <= 0 || (table && tok_seq && slot && k && v && (nh <= 0 || (q && q_out))), "kv_append: null argument");
+    LCU_REQUIRE(table_stride >= 1 && n_seq >= 1 && nkvh >= 1, "kv_append: %d sequences of %d pages, %d KV heads", n_seq, table_stride, nkvh);
+    LCU_REQUIRE(nh == 0 || prep, "kv_append: queries without what to do with them");
+    RowsArgs a{};
+    a.q = q; a.stq = stq; a.shq = shq; a.q_out = q_out; a.stqo = stqo; a.shqo = shqo;
+    a.k = k; a.stk = stk; a.shk = shk; a.v = v; a.stv = stv; a.shv = shv;
+    a.pages = *pages; a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.slot = slot;
+    while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
+    a.pos = pos; a.nh = nh; a.nkvh = nkvh; a.n_v = nkvh; a.dh = dh;
+    return rows_run(a, prep, n, dt, "kv_append", as_stream(s));
+}

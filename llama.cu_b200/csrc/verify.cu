@@ -1,0 +1,507 @@
+// From logits to the tokens that a verified draft leaves (no counterpart in the reference, which samples one token per row,
+// exec/output_head.rs:104-113): probabilities of rows of logits, and the acceptance of drafted tokens against them.
+#include "common.cuh"
+
+namespace lcu {
+
+constexpr int VF_THREADS = 512;
+constexpr int VF_CLUSTER = 8;
+
+__device__ __forceinline__ void vf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void vf_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t vf_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t vf_peer(const void *local, uint32_t cta) {
+    uint32_t la = (uint32_t)__cvta_generic_to_shared(local), ra;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(la), "r"(cta));
+    return ra;
+}
+__device__ __forceinline__ void vf_st_peer(uint32_t ra, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ra), "l"(v) : "memory"); }
+
+template <class T> __device__ __forceinline__ float vf_f(T v) { return Act<T>::to_f(v); }
+template <> __device__ __forceinline__ float vf_f<float>(float v) { return v; }
+
+// ------------------------------------------------------------------ softmax of rows
+//
+//   p_j = exp((x_j - m) / T) / sum_i exp((x_i - m) / T),   m the largest;   T = 0: 1 at the lowest index of the largest, 0 elsewhere
+//
+// Bound by HBM: a row is read once and written once.  A thread-block cluster of up to 8 CTAs takes a row and keeps its values in
+// registers between the two halves (vocabularies up to 131072; longer rows are read a second time, from L2); maxima and sums, relative
+// to each CTA's own maximum, cross the cluster as pairs in one exchange.
+struct SoftmaxArgs {
+    float *probs;
+    size_t stride_p;
+    const void *logits;
+    size_t stride_l;
+    const float *temperature;
+    size_t n, slice;  // values of a row, of a CTA
+};
+
+__device__ __forceinline__ float sm_exp(float x, float m, float inv_t) { return expf((x - m) * inv_t); }
+
+// (value, index) as one number that grows with the value and, among equals, with a lower index; NaN is below everything
+__device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
+    if (!(v == v)) return 0;
+    if (v == 0.f) v = 0.f;  // -0 and 0 are equal
+    const uint32_t b = __float_as_uint(v), u = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return ((unsigned long long)u << 32) | (uint32_t)~i;
+}
+
+template <class T, bool VEC, int EPT>
+__global__ void __launch_bounds__(VF_THREADS) softmax_kernel(const SoftmaxArgs a) {
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    __shared__ unsigned long long part[VF_THREADS / 32], xchg[VF_CLUSTER];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t rank = vf_rank(), size = gridDim.x;
+    const int row = blockIdx.y;
+    vf_cluster_arrive();  // waited for ahead of the exchange: a peer's shared memory is there once it runs
+    const T *x = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.stride_l;
+    float *out = a.probs + (size_t)row * a.stride_p;
+    const size_t lo = (size_t)rank * a.slice < a.n ? (size_t)rank * a.slice : a.n, hi = lo + a.slice < a.n ? lo + a.slice : a.n;
+    const float t = a.temperature ? a.temperature[row] : 1.f;
+    const float inv_t = 1.f / t > 3.0e38f ? 3.0e38f : 1.f / t;  // (x - m) / T stays 0 where x = m, however small T
+
+    auto load = [&](size_t i, float *f) {  // V values from i on; -inf behind the row
+        if (VEC && i + V <= hi) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(x + i);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[k] = __uint_as_float(w[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; k += 2) {
+                    const float2 p = Act<T>::to_f2(w[k / 2]);
+                    f[k] = p.x;
+                    f[k + 1] = p.y;
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[k] = i + k < hi ? vf_f<T>(x[i + k]) : -INFINITY;
+    };
+    auto store = [&](size_t i, const float *f) {
+        if (VEC && i + V <= hi) {
+#pragma unroll
+            for (int k = 0; k < V; k += 4) __stcs(reinterpret_cast<float4 *>(out + i + k), make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]));
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (i + k < hi) __stcs(out + i + k, f[k]);
+    };
+    auto combine = [&](unsigned long long v, auto op) {  // over the block
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (lane == 0) part[warp] = v;
+        __syncthreads();
+        v = part[lane % (VF_THREADS / 32)];
+#pragma unroll
+        for (int o = VF_THREADS / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+        __syncthreads();
+        return v;
+    };
+    auto exchange = [&](unsigned long long v) {  // into everyone's xchg
+        vf_cluster_wait();
+        if (tid < (int)size) vf_st_peer(vf_peer(&xchg[rank], (uint32_t)tid), v);
+        __syncwarp();
+        vf_cluster_arrive();
+        vf_cluster_wait();
+    };
+    auto greater = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
+
+    float keep[EPT > 0 ? EPT : V];
+    const size_t first = lo + (size_t)tid * V, step = (size_t)VF_THREADS * V;
+    if (t == 0.f) {  // (uniform over the cluster)
+        unsigned long long best = 0;
+        for (size_t i = first; i < hi; i += step) {
+            load(i, keep);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (i + k < hi) best = greater(best, sm_key(keep[k], (uint32_t)(i + k)));
+        }
+        exchange(combine(best, greater));
+        best = 0;
+        for (uint32_t c = 0; c < size; ++c) best = greater(best, xchg[c]);
+        // a row of -inf (and NaN) alone has no largest
+        const bool some = (uint32_t)(best >> 32) > 0x007fffffu;
+        const size_t at = some ? (size_t)(uint32_t)~(uint32_t)best : a.n;
+        for (size_t i = first; i < hi; i += step) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) keep[k] = i + k == at ? 1.f : 0.f;
+            store(i, keep);
+        }
+        return;
+    }
+    float m = -INFINITY;
+    if constexpr (EPT > 0) {
+#pragma unroll
+        for (int j = 0; j < EPT / V; ++j) load(first + j * step, keep + j * V);
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) m = fmaxf(m, keep[j]);
+    } else {
+        for (size_t i = first; i < hi; i += step) {
+            load(i, keep);
+#pragma unroll
+            for (int k = 0; k < V; ++k) m = fmaxf(m, keep[k]);
+        }
+    }
+    m = __uint_as_float((uint32_t)combine(__float_as_uint(m), [](unsigned long long p, unsigned long long q) {
+        return (unsigned long long)__float_as_uint(fmaxf(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)q)));
+    }));
+    const float base = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+    if constexpr (EPT > 0) {
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) {
+            keep[j] = sm_exp(keep[j], base, inv_t);
+            s += keep[j];
+        }
+    } else {
+        for (size_t i = first; i < hi; i += step) {
+            load(i, keep);
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += sm_exp(keep[k], base, inv_t);
+        }
+    }
+    s = __uint_as_float((uint32_t)combine(__float_as_uint(s), [](unsigned long long p, unsigned long long q) {
+        return (unsigned long long)__float_as_uint(__uint_as_float((uint32_t)p) + __uint_as_float((uint32_t)q));
+    }));
+    exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s));
+    float top = -INFINITY, sum = 0.f;
+    for (uint32_t c = 0; c < size; ++c) top = fmaxf(top, __uint_as_float((uint32_t)(xchg[c] >> 32)));
+    for (uint32_t c = 0; c < size; ++c) {
+        const float mc = __uint_as_float((uint32_t)(xchg[c] >> 32)), sc = __uint_as_float((uint32_t)xchg[c]);
+        sum += mc == -INFINITY ? sc : sc * sm_exp(mc, top, inv_t);  // (a slice of -inf has sum 0, or NaN where it holds one)
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (EPT > 0) {
+        const float f = (m == -INFINITY ? 1.f : sm_exp(m, top, inv_t)) * inv;
+#pragma unroll
+        for (int j = 0; j < EPT; ++j) keep[j] *= f;
+#pragma unroll
+        for (int j = 0; j < EPT / V; ++j)
+            if (first + j * step < hi) store(first + j * step, keep + j * V);
+    } else {
+        const float b = top == -INFINITY ? 0.f : top;
+        for (size_t i = first; i < hi; i += step) {
+            load(i, keep);
+#pragma unroll
+            for (int k = 0; k < V; ++k) keep[k] = sm_exp(keep[k], b, inv_t) * inv;
+            store(i, keep);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ verification of drafted tokens
+//
+//   draft i of a sequence is accepted while u_i q_i(x_i) < p_i(x_i);
+//   behind the accepted ones comes the first index whose running sum of w exceeds u_last sum(w):
+//   w = max(p - q, 0) at the rejected draft (p itself where nothing is left), w = p behind the last draft
+//
+// in 64 bits, where the products u q and the differences of 32-bit numbers are exact.  Bound by HBM: of all rows only the pair that the last token is drawn
+// from is read whole.  A cluster of up to 8 CTAs takes a sequence: sums of pieces of 512 values or more, totals across the cluster
+// in one exchange, and the CTA that the threshold falls into reads the one piece that holds it again.  The order of the sums is fixed.
+struct VerifyArgs {
+    int32_t *accepted, *tokens;
+    const void *target, *draft;
+    size_t stride_t, stride_d;
+    const int32_t *drafted, *n_drafted;
+    const float *randoms;
+    int k;
+    size_t n, slice, piece;
+};
+
+constexpr int VF_PIECES = 1024;
+
+__device__ __forceinline__ double vf_weight(double p, double q) {
+    const double w = p - q;
+    return w > 0. && w < INFINITY ? w : 0.;  // (NaN and infinities weigh nothing)
+}
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) {
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    __shared__ double piece_sum[VF_PIECES], total[VF_CLUSTER];
+    __shared__ int s_n;
+    __shared__ double s_thr;
+    __shared__ int s_piece;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y, k = a.k;
+    const uint32_t rank = vf_rank(), size = gridDim.x;
+    const T *target = reinterpret_cast<const T *>(a.target) + (size_t)b * (k + 1) * a.stride_t;
+    const T *draft = a.draft ? reinterpret_cast<const T *>(a.draft) + (size_t)b * k * a.stride_d : nullptr;
+    const int32_t *drafted = a.drafted + (size_t)b * k;
+    const float *u = a.randoms + (size_t)b * (k + 1);
+    int32_t *tokens = a.tokens + (size_t)b * (k + 1);
+    vf_cluster_arrive();
+    const int nd = k ? max(0, min(k, a.n_drafted ? a.n_drafted[b] : k)) : 0;
+    auto is_token = [&](int x) { return x >= 0 && (size_t)x < a.n; };
+    if (warp == 0) {
+        int n = nd;
+        for (int i0 = 0; i0 < nd; i0 += 32) {
+            const int i = i0 + lane;
+            bool fine = true;
+            int x = 0;
+            if (i < nd) {
+                x = drafted[i];
+                fine = false;
+                if (is_token(x)) {
+                    const double p = vf_f<T>(target[(size_t)i * a.stride_t + x]), q = draft ? (double)vf_f<T>(draft[(size_t)i * a.stride_d + x]) : 1.;
+                    fine = (double)u[i] * q < p;
+                }
+            }
+            const unsigned bad = __ballot_sync(0xffffffffu, !fine);
+            if (bad) {
+                n = i0 + __ffs(bad) - 1;
+                break;
+            }
+        }
+        if (lane == 0) s_n = n;
+    }
+    __syncthreads();
+    const int n_acc = s_n;
+    const bool held = n_acc < nd;
+    const T *P = target + (size_t)n_acc * a.stride_t, *Q = held && draft ? draft + (size_t)n_acc * a.stride_d : nullptr;
+    const int32_t x_held = held ? drafted[n_acc] : -1;
+    if (rank == 0)
+        for (int i = tid; i <= k; i += VF_THREADS) {
+            if (i == 0) a.accepted[b] = n_acc;
+            if (i != n_acc) tokens[i] = i < n_acc ? drafted[i] : -1;
+        }
+    const size_t lo = (size_t)rank * a.slice < a.n ? (size_t)rank * a.slice : a.n, hi = lo + a.slice < a.n ? lo + a.slice : a.n;
+    const int pieces = (int)((hi - lo + a.piece - 1) / a.piece);
+
+    // weights of V values from i on (i < hi); minus: what the draft gave comes off
+    auto weights = [&](size_t i, bool minus, double *w) {
+        float p[V], q[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[e] = q[e] = 0.f;
+        const bool sub = minus && Q;
+        if (VEC && i + V <= hi) {
+            const uint4 up = *reinterpret_cast<const uint4 *>(P + i), uq = sub ? *reinterpret_cast<const uint4 *>(Q + i) : make_uint4(0, 0, 0, 0);
+            const uint32_t wp[4] = {up.x, up.y, up.z, up.w}, wq[4] = {uq.x, uq.y, uq.z, uq.w};
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) p[e] = __uint_as_float(wp[e]), q[e] = __uint_as_float(wq[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    const float2 f = Act<T>::to_f2(wp[e / 2]), g = Act<T>::to_f2(wq[e / 2]);
+                    p[e] = f.x; p[e + 1] = f.y; q[e] = g.x; q[e + 1] = g.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (i + e < hi) {
+                    p[e] = vf_f<T>(P[i + e]);
+                    if (sub) q[e] = vf_f<T>(Q[i + e]);
+                }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = vf_weight((double)p[e], minus && !Q && (long long)(i + e) == x_held ? 1. : (double)q[e]);
+    };
+    auto sums = [&](bool minus) {  // of the pieces, a warp each; the CTA's total goes to everyone
+        for (int j = warp; j < pieces; j += VF_THREADS / 32) {
+            const size_t p0 = lo + (size_t)j * a.piece, p1 = p0 + a.piece < hi ? p0 + a.piece : hi;
+            double s = 0.;
+            for (size_t i = p0 + (size_t)lane * V; i < p1; i += 32 * V) {
+                double w[V];
+                weights(i, minus, w);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += w[e];
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (lane == 0) piece_sum[j] = s;
+        }
+        __syncthreads();
+        vf_cluster_wait();  // everyone runs, and has read the totals of a first try
+        if (tid == 0) {
+            double s = 0.;
+            for (int j = 0; j < pieces; ++j) s += piece_sum[j];
+            for (uint32_t c = 0; c < size; ++c) vf_st_peer(vf_peer(&total[rank], c), __double_as_longlong(s));
+        }
+        __syncwarp();
+        vf_cluster_arrive();
+        vf_cluster_wait();
+        double all = 0.;
+        for (uint32_t c = 0; c < size; ++c) all += total[c];
+        return all;
+    };
+    bool minus = held;
+    double all = sums(minus);
+    if (minus && !(all > 0.)) {
+        minus = false;
+        vf_cluster_arrive();
+        all = sums(false);
+    }
+    if (!(all > 0.)) {  // a row without mass
+        if (rank == 0 && tid == 0) tokens[n_acc] = -1;
+        return;
+    }
+    // the CTA that the threshold falls into, or the last one with mass
+    const double thr = (double)u[k] * all;
+    double before = 0.;
+    int owner = -1, last = 0;
+    for (uint32_t c = 0; c < size; ++c) {
+        if (total[c] > 0.) last = (int)c;
+        if (owner < 0 && before + total[c] > thr) owner = (int)c;
+        if (owner < 0) before += total[c];
+    }
+    if ((int)rank != (owner < 0 ? last : owner)) return;
+    if (tid == 0) {
+        double run = 0.;
+        int at = 0;
+        for (int j = 0; j < pieces; ++j) {
+            if (!(piece_sum[j] > 0.)) continue;
+            at = j;
+            if (owner >= 0 && before + (run + piece_sum[j]) > thr) break;
+            run += piece_sum[j];
+        }
+        s_piece = at;
+        s_thr = owner >= 0 ? thr - (before + run) : INFINITY;  // what the piece has to reach
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    const size_t p0 = lo + (size_t)s_piece * a.piece, p1 = p0 + a.piece < hi ? p0 + a.piece : hi;
+    const double want = s_thr;
+    double run = 0.;
+    long long found = -1, last_pos = -1;
+    for (size_t i0 = p0; i0 < p1 && found < 0; i0 += 32 * V) {
+        const size_t i = i0 + (size_t)lane * V;
+        double w[V], mine = 0.;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = 0.;
+        if (i < p1) weights(i, minus, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) mine += w[e];
+        double upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        double c = run + (upto - mine);
+        long long hit = -1, pos = -1;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            c += w[e];
+            if (w[e] > 0.) {
+                pos = (long long)(i + e);
+                if (hit < 0 && c > want) hit = pos;
+            }
+        }
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, pos >= 0);
+        if (hits) found = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+        if (some) last_pos = __shfl_sync(0xffffffffu, pos, 31 - __clz(some));
+        run += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) tokens[n_acc] = (int32_t)(found >= 0 ? found : last_pos);
+}
+
+// ------------------------------------------------------------------ host side
+
+template <class... KArgs>
+static int vf_launch(void (*kernel)(KArgs...), int cluster, int rows, cudaStream_t s, KArgs... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster, rows);
+    cfg.blockDim = dim3(VF_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return LCU_OK;
+}
+
+template <class T, bool VEC>
+static int softmax_launch(SoftmaxArgs a, int rows, cudaStream_t s) {
+    // CTAs of a row: as many as give every thread 16 values or more
+    int c = 1;
+    while (c < VF_CLUSTER && a.n > (size_t)c * VF_THREADS * 16) c *= 2;
+    a.slice = ((a.n + c - 1) / c + 7) / 8 * 8;
+    const size_t per = (a.slice + VF_THREADS - 1) / VF_THREADS;
+    for (int r0 = 0; r0 < rows; r0 += 65535) {
+        SoftmaxArgs b = a;
+        b.probs += (size_t)r0 * a.stride_p;
+        b.logits = reinterpret_cast<const T *>(a.logits) + (size_t)r0 * a.stride_l;
+        if (b.temperature) b.temperature += r0;
+        const int m = rows - r0 < 65535 ? rows - r0 : 65535;
+        const int rc = per <= 8 ? vf_launch(softmax_kernel<T, VEC, 8>, c, m, s, (const SoftmaxArgs)b) : per <= 16 ? vf_launch(softmax_kernel<T, VEC, 16>, c, m, s, (const SoftmaxArgs)b)
+                     : per <= 32 ? vf_launch(softmax_kernel<T, VEC, 32>, c, m, s, (const SoftmaxArgs)b) : vf_launch(softmax_kernel<T, VEC, 0>, c, m, s, (const SoftmaxArgs)b);
+        if (rc) return rc;
+    }
+    return LCU_OK;
+}
+
+template <class T>
+static int softmax_t(const SoftmaxArgs &a, int rows, cudaStream_t s) {
+    const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.probs) % 16 == 0 && a.stride_l % (16 / sizeof(T)) == 0 && a.stride_p % 4 == 0;
+    return vec ? softmax_launch<T, true>(a, rows, s) : softmax_launch<T, false>(a, rows, s);
+}
+
+template <class T>
+static int verify_t(VerifyArgs a, int n_seq, cudaStream_t s) {
+    int c = 1;
+    while (c < VF_CLUSTER && a.n > (size_t)c * 4096) c *= 2;
+    a.piece = 512;
+    a.slice = ((a.n + c - 1) / c + 511) / 512 * 512;
+    while (a.slice / a.piece > VF_PIECES) {
+        a.piece *= 2;
+        a.slice = ((a.n + c - 1) / c + a.piece - 1) / a.piece * a.piece;
+    }
+    const bool vec = ((uintptr_t)a.target | (uintptr_t)a.draft) % 16 == 0 && a.stride_t % (16 / sizeof(T)) == 0 && (!a.draft || a.stride_d % (16 / sizeof(T)) == 0);
+    for (int b0 = 0; b0 < n_seq; b0 += 65535) {
+        VerifyArgs v = a;
+        const size_t k = (size_t)a.k;
+        v.accepted += b0;
+        v.tokens += b0 * (k + 1);
+        v.target = reinterpret_cast<const T *>(a.target) + b0 * (k + 1) * a.stride_t;
+        if (a.draft) v.draft = reinterpret_cast<const T *>(a.draft) + b0 * k * a.stride_d;
+        v.drafted += b0 * k;
+        if (a.n_drafted) v.n_drafted += b0;
+        v.randoms += b0 * (k + 1);
+        const int m = n_seq - b0 < 65535 ? n_seq - b0 : 65535;
+        const int rc = vec ? vf_launch(verify_kernel<T, true>, c, m, s, (const VerifyArgs)v) : vf_launch(verify_kernel<T, false>, c, m, s, (const VerifyArgs)v);
+        if (rc) return rc;
+    }
+    return LCU_OK;
+}
+
+}  // namespace lcu
+
+using namespace lcu;
+
+extern "C" int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *logits, size_t stride_l, const float *temperature, int rows, size_t n, int dt,
+                                   lcu_stream_t s) {
+    LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "softmax_rows: dtype %d unsupported", dt);
+    LCU_REQUIRE(rows >= 0 && n >= 1 && n <= 0x7fffffffull && (rows <= 1 || (stride_p >= n && stride_l >= n)), "softmax_rows: %d rows of %zu, strides %zu and %zu", rows,
+                n, stride_l, stride_p);
+    if (rows == 0) return LCU_OK;
+    LCU_REQUIRE(probs && logits, "softmax_rows: null argument");
+    const SoftmaxArgs a{probs, stride_p, logits, stride_l, temperature, n, 0};
+    if (dt == LCU_F16) return softmax_t<__half>(a, rows, as_stream(s));
+    if (dt == LCU_BF16) return softmax_t<__nv_bfloat16>(a, rows, as_stream(s));
+    return softmax_t<float>(a, rows, as_stream(s));
+}
+
+extern "C" int lcu_op_verify_drafts(int32_t *accepted, int32_t *tokens, const void *target, size_t stride_t, const void *draft, size_t stride_d,
+                                    const int32_t *drafted, const int32_t *n_drafted, const float *randoms, int n_seq, int k, size_t n, int dt, lcu_stream_t s) {
+    LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "verify_drafts: dtype %d unsupported", dt);
+    LCU_REQUIRE(n_seq >= 0 && k >= 0 && k <= 0xffff && n >= 1 && n <= 0x7fffffffull, "verify_drafts: %d sequences, %d drafts, %zu tokens", n_seq, k, n);
+    if (n_seq == 0) return LCU_OK;
+    LCU_REQUIRE(accepted && tokens && target && randoms && (k == 0 || drafted), "verify_drafts: null argument");
+    LCU_REQUIRE(stride_t >= n && (!draft || k == 0 || stride_d >= n), "verify_drafts: strides %zu and %zu below %zu", stride_t, stride_d, n);
+    const VerifyArgs a{accepted, tokens, target, k ? draft : nullptr, stride_t, stride_d, drafted, n_drafted, randoms, k, n, 0, 0};
+    if (dt == LCU_F16) return verify_t<__half>(a, n_seq, as_stream(s));
+    if (dt == LCU_BF16) return verify_t<__nv_bfloat16>(a, n_seq, as_stream(s));
+    return verify_t<float>(a, n_seq, as_stream(s));
+}
