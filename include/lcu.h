@@ -560,7 +560,8 @@ LCU_API int lcu_op_kv_append(const lcu_kv_pages *pages, const int32_t *table, in
  * [n, nh, dh]; query head h reads KV head h / (nh / nkvh); scores are scaled by `scale` > 0.  dh 64 or 128, nh / nkvh up to 16, dt LCU_F16 or LCU_BF16.
  * The prefix is read once for all tokens.  f32 scores and softmax, weights rounded to dt ahead of the product with the values, one rounding
  * of the output.  Rows of q, o and the pages start on 16 bytes.  Tokens with tok_seq outside [0, n_seq) are left unwritten; tok_ctx counts at
- * most table_stride pages; positions on page ids that name no page are not seen; a token that sees nothing gets zeros.
+ * most table_stride pages; positions on page ids that name no page are not seen; a token that sees nothing gets zeros.  (Waits inside the
+ * kernel are bounded: rows of one that ran out are NaN.)
  * table may be NULL with table_stride 0: no sequence has pages of its own.  Workspace: lcu_attention_prefix_workspace_size bytes, 256-byte
  * aligned, contents irrelevant (0 bytes: NULL will do). */
 LCU_API size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len);

@@ -1,6 +1,24 @@
 // Attention of a batch whose sequences share a prefix, on a caller's pages (no counterpart in the reference, whose sessions share nothing on the
-// device): softmax over the prefix and the token's own slots together.
+// device): one softmax over the prefix and the token's own slots,
+//
+//   o = sum_j exp(scale q k_j - m) v_j / sum_j exp(scale q k_j - m),   j in the prefix, then in the token's own slots
+//
+// cut where the keys are: partial sums relative to a maximum of their own, (m, l, O), add up as O 2^(m - M), l 2^(m - M).
+//
+//  - prefix_tc_kernel: the prefix, for all tokens at once, on the 5th-generation tensor cores.  The query rows (token, head of the group) of
+//    a KV head fill tiles of 256 rows, so the prefix is read once per 256 rows instead of once per token; the roles, tensor memory and
+//    arithmetic are those of attention_tc.cu.  The units (KV head, row tile, key tile) are dealt to one CTA per SM in equal
+//    contiguous ranges; a CTA leaves one partial result per (KV head, row tile) that it meets.
+//  - own_kernel: each token's own slots, then the sum of all parts.  A CTA owns a KV head and up to 16 query rows of one sequence's
+//    consecutive tokens (drafted tokens share their keys); its four warps take 16 keys each in turns, with a softmax of their own
+//    and both products in registers (mma.sync), and meet once at the end.  It is launched as a programmatic dependent: own slots are worked
+//    on while the prefix runs, and only the sum waits for it.
+//
+// f32 scores and softmax, weights rounded to the activation type ahead of the second product (its operands are 16-bit; the sums are
+// taken over the rounded weights, so the rounding does not shift the whole row), one rounding of the output.
+#include "attention_tc.cuh"
 #include "paged.cuh"
+#include "prefix_plan.hpp"
 
 namespace lcu {
 
@@ -13,88 +31,697 @@ struct PrefixArgs {
     const uint32_t *tok_ctx;
     uint32_t prefix_len;
     int table_stride, n_seq, page_shift, n, nh, nkvh;
-    float scale;
+    float scale2;  // scores in powers of two
+    PrefixPlan plan;
+    float2 *part_ml;  // [slot][row]
+    float *part_o;    // [slot][row][dh]
 };
 
-// One CTA per (query head, token), the keys in turns over its four warps: a key per lane for the scores, dh / 32 dimensions per lane
-// for the output.
+// ------------------------------------------------------------------ the prefix
+
+constexpr int PF_THREADS = 320;
+constexpr int PF_MAX_STAGES = 4;
+
+struct PfShared {
+    unsigned long long k_full[PF_MAX_STAGES], k_empty[PF_MAX_STAGES], v_full[PF_MAX_STAGES], v_empty[PF_MAX_STAGES];
+    unsigned long long q_full[2], s_full[2], p_ready[2], o_done[2], drain;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int DH> constexpr int pf_stages() { return DH == 64 ? 4 : 2; }
+template <int DH> constexpr size_t pf_smem() { return 1024 + (size_t)(DH / 64) * AT_BOX * (2 + 2 * pf_stages<DH>()) + sizeof(PfShared); }
+
+__device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n}"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void pf_st32(float *p, const uint32_t *r) {  // 32 bytes, 16-byte aligned
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// what a CTA does of one (KV head, row tile)
+struct PfPiece {
+    long long unit, end, pair;  // first unit, first unit behind the CTA's range
+    int hkv, row0, rows, j0, j1;
+    bool two;
+};
+__device__ __forceinline__ PfPiece pf_piece(const PrefixPlan &pl, long long unit, long long end) {
+    PfPiece p;
+    p.unit = unit;
+    p.end = end;
+    p.pair = unit / pl.key_tiles;
+    p.j0 = (int)(unit - p.pair * pl.key_tiles);
+    const long long left = end - unit;
+    p.j1 = left < pl.key_tiles - p.j0 ? p.j0 + (int)left : pl.key_tiles;
+    p.hkv = (int)(p.pair / pl.row_tiles);
+    p.row0 = (int)(p.pair - (long long)p.hkv * pl.row_tiles) * PF_ROWS;
+    p.rows = min(PF_ROWS, pl.rows - p.row0);
+    p.two = p.rows > 128;
+    return p;
+}
+__device__ __forceinline__ PfPiece pf_next(const PrefixPlan &pl, const PfPiece &p) { return pf_piece(pl, p.unit + (p.j1 - p.j0), p.end); }
+
 template <class T, int DH>
-__global__ void __launch_bounds__(128) prefix_plain_kernel(const PrefixArgs a) {
-    constexpr int W = 4, PER = DH / 32;
-    __shared__ float qs[DH], part_o[W][DH], part_m[W], part_l[W];
-    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hkv = h / (a.nh / a.nkvh);
-    const int seq = a.tok_seq[t];
-    if (seq < 0 || seq >= a.n_seq) return;
-    const T *q = reinterpret_cast<const T *>(a.q) + (size_t)t * a.stq + (size_t)h * a.shq;
-    for (int i = threadIdx.x; i < DH; i += 128) qs[i] = Act<T>::to_f(q[i]);
-    __syncthreads();
-    const uint32_t cap = (uint32_t)a.table_stride << a.page_shift, own = min(a.tok_ctx[t], cap);
-    const unsigned long long all = (unsigned long long)a.prefix_len + own;
-    auto row = [&](unsigned long long pos) -> long long {
-        const bool shared = pos < a.prefix_len;
-        const uint32_t s = (uint32_t)(shared ? pos : pos - a.prefix_len);
-        const int page = shared ? a.prefix_table[s >> a.page_shift] : a.table[(size_t)seq * a.table_stride + (s >> a.page_shift)];
-        if (page < 0 || page >= a.pages.n_pages) return -1;
-        return (long long)page * a.pages.stride_page + (long long)(s & ((1u << a.page_shift) - 1)) * a.pages.stride_tok + (long long)hkv * a.pages.stride_head;
-    };
-    float m = -INFINITY, l = 0.f, acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-    for (unsigned long long p0 = 32ull * warp; p0 < all; p0 += 32ull * W) {
-        const long long at = p0 + lane < all ? row(p0 + lane) : -1;
-        float s = -INFINITY;
-        if (at >= 0) {
-            s = 0.f;
-            const T *k = reinterpret_cast<const T *>(a.pages.k) + at;
-            for (int i = 0; i < DH; ++i) s = fmaf(qs[i], Act<T>::to_f(k[i]), s);
-            s *= a.scale;
+__global__ void __launch_bounds__(PF_THREADS, 1)
+prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, uint32_t fmt) {
+    constexpr int NB = DH / 64, TILE = NB * AT_BOX, ST = pf_stages<DH>();
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + ((1024u - (tc_smem(smem_raw) & 1023u)) & 1023u);
+    unsigned char *Qs = smem, *Ks = Qs + 2 * TILE, *Vs = Ks + ST * TILE;
+    PfShared *sh = reinterpret_cast<PfShared *>(Vs + ST * TILE);
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    grid_dep_launch();
+    const long long u0 = (long long)blockIdx.x * a.plan.per, u1 = u0 + a.plan.per < a.plan.units ? u0 + a.plan.per : a.plan.units;
+    const int ppt = 128 >> a.page_shift, n_prefix_pages = (int)((a.prefix_len + a.pages.page_tokens - 1) >> a.page_shift);  // pages of a tile, of all
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            tc_mbar_init(tc_smem(&sh->k_full[i]), 1);
+            tc_mbar_init(tc_smem(&sh->k_empty[i]), 1);
+            tc_mbar_init(tc_smem(&sh->v_full[i]), 1);
+            tc_mbar_init(tc_smem(&sh->v_empty[i]), 1);
         }
-        const float mn = fmaxf(m, warp_max(s)), base = mn == -INFINITY ? 0.f : mn, corr = m == -INFINITY ? 0.f : expf(m - base);
-        const float p = s == -INFINITY ? 0.f : expf(s - base);
-        l = l * corr + p;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] *= corr;
-        for (int j = 0; j < 32; ++j) {
-            const long long r = __shfl_sync(0xffffffffu, at, j);
-            const float w = __shfl_sync(0xffffffffu, p, j);
-            if (r < 0) continue;
-            const T *v = reinterpret_cast<const T *>(a.pages.v) + r;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) acc[i] = fmaf(w, Act<T>::to_f(v[lane + 32 * i]), acc[i]);
+        tc_mbar_init(tc_smem(&sh->drain), 1);
+        for (int t = 0; t < 2; ++t) {
+            tc_mbar_init(tc_smem(&sh->q_full[t]), 4);
+            tc_mbar_init(tc_smem(&sh->s_full[t]), 1);
+            tc_mbar_init(tc_smem(&sh->p_ready[t]), 4);
+            tc_mbar_init(tc_smem(&sh->o_done[t]), 1);
         }
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    l = warp_sum(l);
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&sh->tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh->tmem_base, tmem_o = tmem + 256;  // S_t in columns 128 t .., O_t behind them
+    int k_issued = 0, v_issued = 0;  // stages that warp 0 has requested
+
+    if (warp == 0) {
+        // ---------------- TMA producer: the ring runs on through all pieces
+        const uint32_t kf = tc_smem(&sh->k_full[0]), ke = tc_smem(&sh->k_empty[0]), vf = tc_smem(&sh->v_full[0]), ve = tc_smem(&sh->v_empty[0]);
+        const int pt = a.pages.page_tokens;
+        auto page_of = [&](int tile) {  // lane i: page i of the tile; an id that names no page is one behind the map, which reads zeros
+            const int i = tile * ppt + lane;
+            const int id = lane < ppt && i < n_prefix_pages ? a.prefix_table[i] : 0;
+            return id < 0 || id >= a.pages.n_pages ? a.pages.n_pages : id;
+        };
+        int slot = 0, hkv = (int)(u0 / a.plan.key_tiles / a.plan.row_tiles), j = (int)(u0 % a.plan.key_tiles);
+        long long pair = u0 / a.plan.key_tiles;
+        int id = page_of(j);
+        auto load = [&](uint32_t dst, const CUtensorMap *map, uint32_t bar, int n) {
+            tc_warp_expect_tx(bar, (uint32_t)(n * pt * 128 * NB));
+            for (int i = 0; i < n; ++i) {
+                const int page = __shfl_sync(0xffffffffu, id, i);
+                for (int b = 0; b < NB; ++b) pf_tma_4d(dst + (uint32_t)(b * AT_BOX + i * pt * 128), map, 64 * b, 0, hkv, page, bar);
+            }
+        };
+        uint32_t phase = 1;
+        bool ok = true;
+        for (long long u = u0; u < u1; ++u) {
+            const int n = min(ppt, n_prefix_pages - j * ppt);
+            ok = tc_warp_wait(ke + 8 * slot, phase, &sh->abort_flag);
+            if (!ok) break;
+            load(tc_smem(Ks) + (uint32_t)(slot * TILE), &map_k, kf + 8 * slot, n);
+            ++k_issued;
+            ok = tc_warp_wait(ve + 8 * slot, phase, &sh->abort_flag);
+            if (!ok) break;
+            load(tc_smem(Vs) + (uint32_t)(slot * TILE), &map_v, vf + 8 * slot, n);
+            ++v_issued;
+            if (++j == a.plan.key_tiles) {
+                j = 0;
+                ++pair;
+                hkv = (int)(pair / a.plan.row_tiles);
+            }
+            if (u + 1 < u1) id = page_of(j);
+            if (++slot == ST) { slot = 0; phase ^= 1u; }
+        }
+        if (!ok) sh->abort_flag = 1;
+    } else if (warp == 1) {
+        // ---------------- MMA issuer
+        const uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        const uint64_t q0 = tc_desc(tc_smem(Qs)), k0 = tc_desc(tc_smem(Ks)), v0 = at_desc_mn(tc_smem(Vs));
+        const uint32_t kf = tc_smem(&sh->k_full[0]), ke = tc_smem(&sh->k_empty[0]), vf = tc_smem(&sh->v_full[0]), ve = tc_smem(&sh->v_empty[0]);
+        const uint32_t sf = tc_smem(&sh->s_full[0]), pr = tc_smem(&sh->p_ready[0]), od = tc_smem(&sh->o_done[0]), qf = tc_smem(&sh->q_full[0]);
+        auto scores = [&](int t, int slot) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) part_o[warp][lane + 32 * i] = acc[i];
-    if (lane == 0) {
-        part_m[warp] = m;
-        part_l[warp] = l;
+            for (int b = 0; b < NB; ++b)
+                tc_warp_mma4(tmem + 128 * t, q0 + (uint64_t)((t * TILE + b * AT_BOX) >> 4), k0 + (uint64_t)((slot * TILE + b * AT_BOX) >> 4), id_s, b > 0);
+            tc_warp_commit(sf + 8 * t);
+        };
+        int slot = 0;
+        uint32_t phase = 0, p_phase = 0, q_phase = 0;  // bit t of the last two: tile t's
+        bool ok = true;
+        for (PfPiece p = pf_piece(a.plan, u0, u1); ok && p.unit < u1; p = pf_next(a.plan, p)) {
+            const int nt = p.two ? 2 : 1;
+            for (int t = 0; t < nt && ok; ++t) {
+                ok = tc_warp_wait(qf + 8 * t, q_phase >> t & 1u, &sh->abort_flag);
+                q_phase ^= 1u << t;
+            }
+            ok = ok && tc_warp_wait(kf + 8 * slot, phase, &sh->abort_flag);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int t = 0; t < nt; ++t) scores(t, slot);
+            tc_warp_commit(ke + 8 * slot);
+            for (int j = p.j0; j < p.j1 && ok; ++j) {
+                const int next = slot + 1 == ST ? 0 : slot + 1;
+                const uint32_t next_phase = slot + 1 == ST ? phase ^ 1u : phase;
+                const bool more = j + 1 < p.j1;
+                ok = tc_warp_wait(vf + 8 * slot, phase, &sh->abort_flag);
+                if (ok && more) ok = tc_warp_wait(kf + 8 * next, next_phase, &sh->abort_flag);
+                for (int t = 0; t < nt && ok; ++t) {
+                    ok = tc_warp_wait(pr + 8 * t, p_phase >> t & 1u, &sh->abort_flag);
+                    p_phase ^= 1u << t;
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)  // 16 positions: 8 columns of weights, 2 KB of the V tile
+                        at_mma_ts(tmem_o + DH * t, tmem + 128 * t + 8 * k, v0 + (uint64_t)((slot * TILE + k * 2048) >> 4), id_o, j > p.j0 || k > 0);
+                    if (t == nt - 1) tc_warp_commit(ve + 8 * slot);
+                    if (more) {
+                        scores(t, next);
+                        if (t == nt - 1) tc_warp_commit(ke + 8 * next);
+                    } else {
+                        tc_warp_commit(od + 8 * t);
+                    }
+                }
+                slot = next;
+                phase = next_phase;
+            }
+        }
+        if (!ok) sh->abort_flag = 1;
+    } else {
+        // ---------------- queries, softmax and partial output of one tile: a row per thread
+        const int t = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;  // a warp may only touch TMEM lanes [32 q, 32 q + 32)
+        const int group = a.nh / a.nkvh;
+        const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + 128 * t, to = tmem_o + ((uint32_t)(q * 32) << 16) + DH * t;
+        auto load_q = [&](const PfPiece &p) {  // 16 bytes per thread and step, as the 128-byte swizzle has them; zeros behind the last row
+            constexpr int CH = DH / 8;
+            const int i = tid - 64 - 128 * t;
+#pragma unroll 4
+            for (int k = 0; k < CH; ++k) {
+                const int r = i / CH + k * (128 / CH), c = i % CH, at = 128 * t + r;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (at < p.rows) {
+                    const int tok = (p.row0 + at) / group, g = p.row0 + at - tok * group;
+                    u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + (size_t)tok * a.stq + (size_t)(p.hkv * group + g) * a.shq + 8 * c);
+                }
+                *reinterpret_cast<uint4 *>(Qs + t * TILE + (c >> 3) * AT_BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(&sh->q_full[t])) : "memory");
+        };
+        auto bad_pages = [&](int tile) {  // bit i: page i of the tile names no page
+            const int i = tile * ppt + lane;
+            const int id = lane < ppt && i < n_prefix_pages ? a.prefix_table[i] : 0;
+            return __ballot_sync(0xffffffffu, id < 0 || id >= a.pages.n_pages);
+        };
+        int it = 0;          // units of the CTA so far
+        uint32_t mine = 0;   // ... that had this tile
+        uint32_t pieces = 0;
+        bool ok = true;
+        PfPiece p = pf_piece(a.plan, u0, u1);
+        if (t == 0 || p.two) load_q(p);
+        while (p.unit < u1) {
+            const bool active = t == 0 || p.two, some = active && 128 * t + q * 32 < p.rows;  // ... of this warp's rows
+            float ref = -INFINITY, l = 0.f;
+            if (active) {
+                unsigned bad = bad_pages(p.j0);
+                for (int j = p.j0; j < p.j1; ++j, ++mine) {
+                    const int p0 = j * 128, left = (int)min((long long)a.prefix_len - p0, 128ll);
+                    if (t == 0 && left < 128) {  // V rows behind the prefix: whatever a page holds there has weight zero
+                        const int u = it + (j - p.j0), slot = u % ST;
+                        ok = tc_mbar_wait(tc_smem(&sh->v_full[slot]), (uint32_t)(u / ST) & 1u, &sh->abort_flag);
+                        uint4 *v = reinterpret_cast<uint4 *>(Vs + (size_t)slot * TILE);
+                        for (int i = left * 8 + (tid - 64); ok && i < 128 * 8; i += 128)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) v[b * (AT_BOX / 16) + i] = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    ok = ok && tc_mbar_wait(tc_smem(&sh->s_full[t]), mine & 1u, &sh->abort_flag);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    const unsigned hide = bad;
+                    if (j + 1 < p.j1) bad = bad_pages(j + 1);
+                    if (some) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        uint32_t s[128];
+#pragma unroll
+                        for (int c = 0; c < 128; c += 32) at_ld32(ts + c, s + c);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (left < 128 || hide) {
+#pragma unroll
+                            for (int c = 0; c < 128; ++c)
+                                if (c >= left || (hide >> (c >> a.page_shift) & 1u)) s[c] = 0xff800000u;
+                        }
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 0; c < 128; c += 8)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) m4[i] = at_max3(m4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
+                        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale2;
+                        if (__any_sync(0xffffffffu, m > ref)) {
+                            const float mn = fmaxf(ref, m), corr = ref == -INFINITY ? 0.f : at_exp2(ref - mn);
+                            l *= corr;
+                            ref = mn;
+                            if (j > p.j0) {
+#pragma unroll 1
+                                for (int c = 0; c < DH; c += 16) {
+                                    uint32_t o[16];
+                                    tc_ld16(to + c, o);
+                                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                                    at_st16(to + c, o);
+                                }
+                            }
+                        }
+                        const float sub = ref == -INFINITY ? 0.f : ref;  // a row whose scores are all -inf keeps zero weights
+                        const unsigned long long mul = at_pair(a.scale2, a.scale2), off = at_pair(-sub, -sub);
+                        unsigned long long l2[2] = {0ull, 0ull};
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int c = 32 * h + 2 * i;
+                                const float2 x = at_unpair(at_fma2(at_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul, off));
+                                w[i] = Act<T>::pack(at_exp2(x.x), at_exp2(x.y));
+                                const float2 f = Act<T>::to_f2(w[i]);
+                                l2[i & 1] = at_add2(l2[i & 1], at_pair(f.x, f.y));
+                            }
+                            at_st16(ts + 16 * h, w);
+                        }
+                        const float2 la = at_unpair(at_add2(l2[0], l2[1]));
+                        l += la.x + la.y;
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(&sh->p_ready[t])) : "memory");
+                }
+                if (!ok) break;
+            }
+            it += p.j1 - p.j0;
+            const PfPiece next = pf_next(a.plan, p);
+            // the products of this tile's scores have ended (their last commit was waited for): its queries may be replaced
+            if (next.unit < u1 && (t == 0 || next.two)) load_q(next);
+            if (active) {
+                ok = tc_mbar_wait(tc_smem(&sh->o_done[t]), pieces & 1u, &sh->abort_flag);
+                ++pieces;
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const size_t at = (size_t)(blockIdx.x + p.pair) * a.plan.slot_rows + 128 * t + row;
+                const bool valid = 128 * t + row < p.rows;
+                if (valid) a.part_ml[at] = make_float2(ref, l);
+                if (some) {
+#pragma unroll
+                    for (int c = 0; c < DH; c += 32) {
+                        uint32_t o[32];
+                        at_ld32(to + c, o);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (!valid) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) pf_st32(a.part_o + at * DH + c + i, o + i);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            }
+            p = next;
+        }
+        if (!ok) sh->abort_flag = 1;
     }
     __syncthreads();
-    float top = -INFINITY, sum = 0.f, f[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, part_m[w]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        f[w] = part_m[w] == -INFINITY ? 0.f : expf(part_m[w] - top);
-        sum += part_l[w] * f[w];
+    if (sh->abort_flag) {  // a wait has run out: what still writes to the CTA's memory ends first, and the rows it had become NaN
+        if (warp == 0) {
+            tc_warp_drain_ring(tc_smem(&sh->k_full[0]), k_issued, ST);
+            tc_warp_drain_ring(tc_smem(&sh->v_full[0]), v_issued, ST);
+        }
+        if (warp == 1) {
+            tc_warp_commit(tc_smem(&sh->drain));
+            tc_warp_drain(tc_smem(&sh->drain), 0u);
+        }
+        for (PfPiece p = pf_piece(a.plan, u0, u1); p.unit < u1; p = pf_next(a.plan, p))
+            for (int r = tid; r < p.rows; r += PF_THREADS) a.part_ml[(size_t)(blockIdx.x + p.pair) * a.plan.slot_rows + r] = make_float2(0.f, __int_as_float(0x7fc00000));
+        __syncthreads();
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T *o = reinterpret_cast<T *>(a.o) + (size_t)t * a.sto + (size_t)h * a.sho;
-    for (int i = threadIdx.x; i < DH; i += 128) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) v = fmaf(part_o[w][i], f[w], v);
-        o[i] = Act<T>::from_f(v * inv);
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
 }
 
-template <class T>
-static int prefix_run(const PrefixArgs &a, int dh, cudaStream_t s) {
-    if (dh == 64) prefix_plain_kernel<T, 64><<<dim3(a.nh, a.n), 128, 0, s>>>(a);
-    else prefix_plain_kernel<T, 128><<<dim3(a.nh, a.n), 128, 0, s>>>(a);
-    LCU_CHECK_CUDA(cudaGetLastError());
+// ------------------------------------------------------------------ own slots, and the sum
+
+constexpr int OW_KEYS = 16, OW_WARPS = 4, OW_THREADS = 32 * OW_WARPS, OW_STAGES = 2;
+
+template <int DH> constexpr size_t ow_stage_bytes() { return (size_t)2 * OW_KEYS * (DH + 8) * 2; }
+template <int DH> constexpr size_t ow_smem() { return OW_WARPS * OW_STAGES * ow_stage_bytes<DH>(); }  // later the warps' parts: 16 rows of DH f32 each
+template <int DH> constexpr size_t ow_part_bytes() { return (size_t)16 * DH * 4 + 16 * 8; }        // a CTA's part in the first one's memory (clusters)
+
+__device__ __forceinline__ void ow_cp16(void *dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ow_ldm4(uint32_t r[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((uint32_t)__cvta_generic_to_shared(p)) : "memory");
+}
+__device__ __forceinline__ void ow_ldm4t(uint32_t r[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((uint32_t)__cvta_generic_to_shared(p)) : "memory");
+}
+__device__ __forceinline__ float ow_quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float ow_quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// factor of a part (m, l, O) in a sum relative to M: a part without a maximum has l = 0 and O = 0, or NaN, which stays
+__device__ __forceinline__ float ow_factor(float m, float M) { return m == -INFINITY ? 1.f : at_exp2(m - M); }
+
+// grid (splits, KV heads, tokens), the splits of a token a cluster
+template <class T, int DH>
+__global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int tokens_per, int splits) {
+    constexpr int ROW = DH + 8, KS = DH / 16, PD = DH / 32;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float ml[OW_WARPS][16][2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t4 = lane & 3;
+    const int hkv = blockIdx.y, t = blockIdx.z, split = blockIdx.x, group = a.nh / a.nkvh;
+    const bool first_block = (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
+    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of stores to the first CTA
+    // consecutive tokens of one sequence, cut at multiples of tokens_per
+    const int seq = a.tok_seq[t];
+    const bool mine = seq >= 0 && seq < a.n_seq && (t % tokens_per == 0 || a.tok_seq[t - 1] != seq);
+    if (!mine) {
+        if (splits > 1) {
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        }
+        if (first_block) grid_dep_wait();  // one block at least ends behind the prefix
+        return;
+    }
+    const int most = min(tokens_per - t % tokens_per, a.n - t);
+    const unsigned same = __ballot_sync(0xffffffffu, lane < most && a.tok_seq[t + min(lane, most - 1)] == seq);
+    const int n_tok = __ffs(~same) - 1, rows = n_tok * group;  // most <= 16: there is a zero
+    const uint32_t cap = (uint32_t)a.table_stride << a.page_shift;
+    uint32_t ctx = 0;  // of the longest
+    if (lane < n_tok) ctx = min(a.tok_ctx[t + lane], cap);
+    const uint32_t r0 = (uint32_t)gid, r1 = r0 + 8;  // this thread's rows
+    const uint32_t lim0 = __shfl_sync(0xffffffffu, ctx, (int)(r0 / group) & 31), lim1 = __shfl_sync(0xffffffffu, ctx, (int)(r1 / group) & 31);
+    const uint32_t lim_min = __reduce_min_sync(0xffffffffu, lane < n_tok ? ctx : 0xffffffffu);
+    ctx = __reduce_max_sync(0xffffffffu, ctx);
+    const int chunks = (int)((ctx + OW_KEYS - 1) / OW_KEYS);
+
+    uint32_t qa[KS][4];
+    {
+        auto row_of = [&](int r) { return reinterpret_cast<const T *>(a.q) + (size_t)(t + r / group) * a.stq + (size_t)(hkv * group + r % group) * a.shq; };
+        const T *q0 = row_of((int)r0 < rows ? (int)r0 : 0), *q1 = row_of((int)r1 < rows ? (int)r1 : 0);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            qa[k][0] = *reinterpret_cast<const uint32_t *>(q0 + 16 * k + 2 * t4);
+            qa[k][1] = *reinterpret_cast<const uint32_t *>(q1 + 16 * k + 2 * t4);
+            qa[k][2] = *reinterpret_cast<const uint32_t *>(q0 + 16 * k + 8 + 2 * t4);
+            qa[k][3] = *reinterpret_cast<const uint32_t *>(q1 + 16 * k + 8 + 2 * t4);
+        }
+    }
+    unsigned char *ring = smem + (size_t)warp * OW_STAGES * ow_stage_bytes<DH>();
+    const int step = splits * OW_WARPS;
+    auto row_at = [&](int chunk) -> long long {  // lane i: where key i of the chunk lies, -1: nowhere
+        const uint32_t key = (uint32_t)chunk * OW_KEYS + (lane & 15);
+        if (chunk >= chunks || key >= ctx) return -1;
+        const int page = a.table[(size_t)seq * a.table_stride + (key >> a.page_shift)];
+        if (page < 0 || page >= a.pages.n_pages) return -1;
+        return (long long)page * a.pages.stride_page + (long long)(key & ((1u << a.page_shift) - 1)) * a.pages.stride_tok + (long long)hkv * a.pages.stride_head;
+    };
+    auto request = [&](int stage, long long at) {
+        T *ks = reinterpret_cast<T *>(ring + (size_t)stage * ow_stage_bytes<DH>()), *vs = ks + OW_KEYS * ROW;
+        constexpr int CH = DH / 8;
+#pragma unroll
+        for (int i = 0; i < OW_KEYS * CH / 32; ++i) {
+            const int key = lane / CH + i * (32 / CH), c = 8 * (lane % CH);
+            const long long off = __shfl_sync(0xffffffffu, at, key);
+            ow_cp16(ks + key * ROW + c, reinterpret_cast<const T *>(a.pages.k) + (off < 0 ? 0 : off + c), off >= 0);
+            ow_cp16(vs + key * ROW + c, reinterpret_cast<const T *>(a.pages.v) + (off < 0 ? 0 : off + c), off >= 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float o[DH / 8][4];
+#pragma unroll
+    for (int i = 0; i < DH / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    const int c0 = split * OW_WARPS + warp;
+    long long at = row_at(c0), ahead = row_at(c0 + step);
+    unsigned there = __ballot_sync(0xffffffffu, at >= 0);
+    if (c0 < chunks) request(0, at);
+    int stage = 0;
+    for (int c = c0; c < chunks; c += step) {
+        at = ahead;
+        ahead = row_at(c + 2 * step);
+        const unsigned there_next = __ballot_sync(0xffffffffu, at >= 0);
+        if (c + step < chunks) {
+            request(stage ^ 1, at);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncwarp();
+        const T *ks = reinterpret_cast<const T *>(ring + (size_t)stage * ow_stage_bytes<DH>()), *vs = ks + OW_KEYS * ROW;
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t b[4];
+            ow_ldm4(b, ks + ((lane & 7) + (lane >> 4) * 8) * ROW + 16 * k + (lane >> 3 & 1) * 8);
+            mma16816<T>(s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[0], b[1]);
+            mma16816<T>(s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[2], b[3]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = 8 * h + 2 * t4 + e;
+                const uint32_t key = (uint32_t)c * OW_KEYS + i;
+                const bool seen = there >> i & 1u;
+                s[h][e] = seen && key < lim0 ? s[h][e] * a.scale2 : -INFINITY;
+                s[h][2 + e] = seen && key < lim1 ? s[h][2 + e] * a.scale2 : -INFINITY;
+            }
+        const float n0 = fmaxf(m0, ow_quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]))));
+        const float n1 = fmaxf(m1, ow_quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]))));
+        const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+        const float f0 = m0 == -INFINITY ? 0.f : at_exp2(m0 - b0), f1 = m1 == -INFINITY ? 0.f : at_exp2(m1 - b1);
+        m0 = n0;
+        m1 = n1;
+        uint32_t pa[4];
+        pa[0] = Act<T>::pack(at_exp2(s[0][0] - b0), at_exp2(s[0][1] - b0));
+        pa[1] = Act<T>::pack(at_exp2(s[0][2] - b1), at_exp2(s[0][3] - b1));
+        pa[2] = Act<T>::pack(at_exp2(s[1][0] - b0), at_exp2(s[1][1] - b0));
+        pa[3] = Act<T>::pack(at_exp2(s[1][2] - b1), at_exp2(s[1][3] - b1));
+        const float2 w0 = Act<T>::to_f2(pa[0]), w1 = Act<T>::to_f2(pa[1]), w2 = Act<T>::to_f2(pa[2]), w3 = Act<T>::to_f2(pa[3]);
+        l0 = l0 * f0 + ((w0.x + w0.y) + (w2.x + w2.y));
+        l1 = l1 * f1 + ((w1.x + w1.y) + (w3.x + w3.y));
+        if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < DH / 8; ++i) {
+                o[i][0] *= f0;
+                o[i][1] *= f0;
+                o[i][2] *= f1;
+                o[i][3] *= f1;
+            }
+        }
+        // Keys that one token of the group sees and another does not: a weight of zero times a value that is not finite would be NaN.
+        bool odd = false;
+        if ((uint32_t)(c + 1) * OW_KEYS > lim_min && lim_min < ctx)
+            for (int i = lane; i < OW_KEYS * DH / 2; i += 32) {
+                const float2 v = Act<T>::to_f2(*reinterpret_cast<const uint32_t *>(vs + i / (DH / 2) * ROW + i % (DH / 2) * 2));
+                odd = odd || !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY);
+            }
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+            for (int i = 0; i < OW_KEYS; ++i) {
+                const int from = (lane & ~3) | (i & 7) >> 1;  // the lane that has the weights of key i
+                const float2 u0 = Act<T>::to_f2(__shfl_sync(0xffffffffu, i < 8 ? pa[0] : pa[2], from)), u1 = Act<T>::to_f2(__shfl_sync(0xffffffffu, i < 8 ? pa[1] : pa[3], from));
+                const float x0 = i & 1 ? u0.y : u0.x, x1 = i & 1 ? u1.y : u1.x;
+                const uint32_t key = (uint32_t)c * OW_KEYS + i;
+                const bool seen = there >> i & 1u;
+#pragma unroll
+                for (int d = 0; d < DH / 8; ++d) {
+                    const float2 v = Act<T>::to_f2(*reinterpret_cast<const uint32_t *>(vs + i * ROW + 8 * d + 2 * t4));
+                    if (seen && key < lim0) {
+                        o[d][0] = fmaf(x0, v.x, o[d][0]);
+                        o[d][1] = fmaf(x0, v.y, o[d][1]);
+                    }
+                    if (seen && key < lim1) {
+                        o[d][2] = fmaf(x1, v.x, o[d][2]);
+                        o[d][3] = fmaf(x1, v.y, o[d][3]);
+                    }
+                }
+            }
+        } else
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) {
+            uint32_t b[4];
+            ow_ldm4t(b, vs + (lane & 15) * ROW + 16 * i + (lane >> 4) * 8);
+            mma16816<T>(o[2 * i], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+            mma16816<T>(o[2 * i + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+        }
+        __syncwarp();  // the stage may be filled again
+        there = there_next;
+        stage ^= 1;
+    }
+    l0 = ow_quad_sum(l0);
+    l1 = ow_quad_sum(l1);
+    __syncthreads();  // the rings are done with: the warps' parts go there
+    float *parts = reinterpret_cast<float *>(smem);  // [warp][16][DH]
+    if (t4 == 0) {
+        ml[warp][gid][0] = m0;
+        ml[warp][gid][1] = l0;
+        ml[warp][gid + 8][0] = m1;
+        ml[warp][gid + 8][1] = l1;
+    }
+#pragma unroll
+    for (int i = 0; i < DH / 8; ++i) {
+        float *d = parts + ((size_t)warp * 16 + gid) * DH + 8 * i + 2 * t4;
+        *reinterpret_cast<float2 *>(d) = make_float2(o[i][0], o[i][1]);
+        *reinterpret_cast<float2 *>(d + 8 * DH) = make_float2(o[i][2], o[i][3]);
+    }
+    __syncthreads();
+    // a warp per row from here on, PD values per lane
+    struct Part {
+        float m, l, o[PD];
+    };
+    auto add = [&](Part &p, float m, float l, const float *v) {  // v: this lane's PD values
+        const float M = fmaxf(p.m, m), f = ow_factor(p.m, M), g = ow_factor(m, M);
+        p.m = M;
+        p.l = p.l * f + l * g;
+#pragma unroll
+        for (int i = 0; i < PD; ++i) p.o[i] = p.o[i] * f + v[i] * g;
+    };
+    float *cluster_o = reinterpret_cast<float *>(smem + ow_smem<DH>());  // first split: [split][16][DH], then (m, l) [split][16]
+    float *cluster_ml = cluster_o + (size_t)splits * 16 * DH;
+    if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    Part held[16 / OW_WARPS];
+#pragma unroll
+    for (int k = 0; k < 16 / OW_WARPS; ++k) {
+        const int r = warp + OW_WARPS * k;
+        Part &p = held[k];
+        p.m = -INFINITY;
+        p.l = 0.f;
+#pragma unroll
+        for (int i = 0; i < PD; ++i) p.o[i] = 0.f;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int w = 0; w < OW_WARPS; ++w) add(p, ml[w][r][0], ml[w][r][1], parts + ((size_t)w * 16 + r) * DH + lane * PD);
+        if (splits > 1) {
+            uint32_t peer;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"((uint32_t)__cvta_generic_to_shared(cluster_o + ((size_t)split * 16 + r) * DH + lane * PD)), "r"(0));
+#pragma unroll
+            for (int i = 0; i < PD; ++i) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer + 4 * i), "f"(p.o[i]) : "memory");
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"((uint32_t)__cvta_generic_to_shared(cluster_ml + ((size_t)split * 16 + r) * 2)), "r"(0));
+            if (lane == 0) asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer), "f"(p.m), "f"(p.l) : "memory");
+        }
+    }
+    if (splits > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (split != 0) return;
+#pragma unroll
+        for (int k = 0; k < 16 / OW_WARPS; ++k) {
+            const int r = warp + OW_WARPS * k;
+            if (r >= rows) continue;
+            for (int s = 1; s < splits; ++s) add(held[k], cluster_ml[(s * 16 + r) * 2], cluster_ml[(s * 16 + r) * 2 + 1], cluster_o + ((size_t)s * 16 + r) * DH + lane * PD);
+        }
+    }
+    grid_dep_wait();  // the parts of the prefix
+#pragma unroll
+    for (int k = 0; k < 16 / OW_WARPS; ++k) {
+        const int r = warp + OW_WARPS * k;
+        if (r >= rows) continue;
+        Part &p = held[k];
+        const int tok = t + r / group, g = r % group;
+        if (a.prefix_len) {
+            const int row = tok * group + g;  // of the KV head
+            const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, last = a.plan.last_cta(pair);
+            for (long long c = a.plan.first_cta(pair); c <= last; ++c) {
+                const size_t at = (size_t)(c + pair) * a.plan.slot_rows + row % PF_ROWS;
+                const float2 x = __ldcg(a.part_ml + at);
+                float v[PD];
+                if constexpr (PD == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at * DH) + lane);
+                    v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+                } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(a.part_o + at * DH) + lane);
+                    v[0] = y.x; v[1] = y.y;
+                }
+                add(p, x.x, x.y, v);
+            }
+        }
+        const float inv = p.l == 0.f ? 0.f : 1.f / p.l;
+        T *dst = reinterpret_cast<T *>(a.o) + (size_t)tok * a.sto + (size_t)(hkv * group + g) * a.sho + lane * PD;
+#pragma unroll
+        for (int i = 0; i < PD; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = Act<T>::pack(p.o[i] * inv, p.o[i + 1] * inv);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+static int pf_map(CUtensorMap *m, int dt, const void *base, const lcu_kv_pages &p, int dh, int nkvh) {
+    const cuuint64_t dims[4] = {(cuuint64_t)dh, (cuuint64_t)p.page_tokens, (cuuint64_t)nkvh, (cuuint64_t)p.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.stride_tok * 2, (cuuint64_t)p.stride_head * 2, (cuuint64_t)p.stride_page * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.page_tokens, 1, 1}, es[4] = {1, 1, 1, 1};
+    LCU_REQUIRE(tc_encode_fn(), "attention_prefix: no cuTensorMapEncodeTiled");
+    const CUresult r = tc_encode_fn()(m, dt == LCU_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), dims, strides,
+                                      box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    LCU_REQUIRE(r == CUDA_SUCCESS, "attention_prefix: cuTensorMapEncodeTiled failed with %d", (int)r);
+    return LCU_OK;
+}
+
+template <class T, int DH>
+static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
+    if (a.prefix_len) {
+        CUtensorMap mk, mv;
+        int rc = pf_map(&mk, dt, a.pages.k, a.pages, DH, a.nkvh);
+        if (!rc) rc = pf_map(&mv, dt, a.pages.v, a.pages, DH, a.nkvh);
+        if (rc) return rc;
+        LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem<DH>()));
+        LCU_CHECK_CUDA(launch_kernel(prefix_tc_kernel<T, DH>, dim3(a.plan.ctas), dim3(PF_THREADS), pf_smem<DH>(), s, false, a, mk, mv, dt == LCU_BF16 ? 1u : 0u));
+    }
+    const int group = a.nh / a.nkvh, tokens_per = 16 / group;
+    // long contexts of few tokens: their keys over a cluster
+    const long long cap = (long long)a.table_stride << a.page_shift, blocks = (long long)a.nkvh * a.n;
+    int splits = 1;
+    while (splits < 8 && blocks * splits * 2 <= 2LL * sm_count() && cap > (long long)splits * 128) splits *= 2;
+    const size_t smem = ow_smem<DH>() + (splits > 1 ? splits * ow_part_bytes<DH>() : 0);
+    LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>() + 8 * ow_part_bytes<DH>())));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, a.nkvh, a.n);
+    cfg.blockDim = dim3(OW_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int n_attr = 0;
+    if (splits > 1) {
+        attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+        attr[n_attr].val.clusterDim.x = splits;
+        attr[n_attr].val.clusterDim.y = attr[n_attr].val.clusterDim.z = 1;
+        ++n_attr;
+    }
+    if (a.prefix_len) {
+        attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+        ++n_attr;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n_attr;
+    LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, own_kernel<T, DH>, (const PrefixArgs)a, tokens_per, splits));
     return LCU_OK;
 }
 
@@ -103,8 +730,8 @@ static int prefix_run(const PrefixArgs &a, int dh, cudaStream_t s) {
 using namespace lcu;
 
 extern "C" size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len) {
-    (void)n, (void)nh, (void)nkvh, (void)dh, (void)prefix_len;
-    return 0;
+    if (n <= 0 || nkvh <= 0 || nh < nkvh || nh % nkvh || dh <= 0 || !prefix_len) return 0;
+    return prefix_bytes(prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count()), dh);
 }
 
 extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q, int stq, int shq, const lcu_kv_pages *pages, const int32_t *prefix_table,
@@ -123,7 +750,7 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     if (n == 0) return LCU_OK;
     LCU_REQUIRE(o && q && tok_seq && tok_ctx && (prefix_table || !prefix_len) && (table || !table_stride), "attention_prefix: null argument");
     LCU_REQUIRE((((uintptr_t)o | (uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v) % 16) == 0 && (sto | sho | stq | shq) % 8 == 0 &&
-                    pages->stride_page % 8 == 0 && pages->stride_tok % 8 == 0 && pages->stride_head % 8 == 0,
+                    pages->stride_page % 8 == 0 && pages->stride_tok % 8 == 0 && pages->stride_head % 8 == 0 && pages->stride_head > 0,
                 "attention_prefix: rows of q, o and the pages start on 16 bytes");
     const size_t need = lcu_attention_prefix_workspace_size(n, nh, nkvh, dh, prefix_len);
     LCU_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0 && workspace_len >= need), "attention_prefix: workspace of %zu bytes, %zu needed (256-byte aligned)",
@@ -133,6 +760,12 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     a.pages = *pages; a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.tok_ctx = tok_ctx;
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
-    a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale = scale;
-    return dt == LCU_F16 ? prefix_run<__half>(a, dh, as_stream(s)) : prefix_run<__nv_bfloat16>(a, dh, as_stream(s));
+    a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale * 1.4426950408889634f;
+    if (prefix_len) {
+        a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count());
+        a.part_ml = reinterpret_cast<float2 *>(workspace);
+        a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan));
+    }
+    if (dt == LCU_F16) return dh == 64 ? prefix_run<__half, 64>(a, dt, as_stream(s)) : prefix_run<__half, 128>(a, dt, as_stream(s));
+    return dh == 64 ? prefix_run<__nv_bfloat16, 64>(a, dt, as_stream(s)) : prefix_run<__nv_bfloat16, 128>(a, dt, as_stream(s));
 }

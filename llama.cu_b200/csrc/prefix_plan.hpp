@@ -1,0 +1,49 @@
+// How the attention of a shared prefix is cut: host and device arithmetic, no GPU needed.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define LCU_HD __host__ __device__
+#else
+#define LCU_HD
+#endif
+
+namespace lcu {
+
+constexpr int PF_ROWS = 256, PF_TILE = 128;  // query rows of a row tile (two MMA tiles), positions of a key tile
+
+// The units (KV head, row tile, key tile) in this order are dealt to the CTAs in equal contiguous ranges; what a CTA does of one
+// (KV head, row tile) is a piece with a partial result of its own.  CTA c's piece of pair p has number c + p: both only grow along the
+// units, and each piece begins a new CTA or a new pair, so no two pieces share a number.
+struct PrefixPlan {
+    int rows;        // query rows of a KV head: tokens x heads of its group
+    int row_tiles, key_tiles;
+    long long pairs, units, per;  // (KV head, row tile); all units; units of a CTA
+    int ctas;
+    int slot_rows;   // rows of a piece's slot
+
+    LCU_HD long long first_cta(long long pair) const { return pair * key_tiles / per; }
+    LCU_HD long long last_cta(long long pair) const { return ((pair + 1) * key_tiles - 1) / per; }
+    LCU_HD long long slots() const { return ctas + pairs; }
+};
+
+// n tokens, `group` query heads per KV head, a prefix of prefix_len > 0 positions, at most `sms` CTAs
+inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, int sms) {
+    PrefixPlan p;
+    p.rows = n * group;
+    p.row_tiles = (p.rows + PF_ROWS - 1) / PF_ROWS;
+    p.key_tiles = (int)((prefix_len + PF_TILE - 1) / PF_TILE);
+    p.pairs = (long long)nkvh * p.row_tiles;
+    p.units = p.pairs * p.key_tiles;
+    p.per = (p.units + sms - 1) / sms;
+    p.ctas = (int)((p.units + p.per - 1) / p.per);
+    p.slot_rows = p.rows < PF_ROWS ? p.rows : PF_ROWS;
+    return p;
+}
+
+// Workspace: (maximum, sum) of every row of every slot, then the rows' unnormalised outputs.
+inline size_t prefix_ml_bytes(const PrefixPlan &p) { return ((size_t)p.slots() * p.slot_rows * 8 + 255) / 256 * 256; }
+inline size_t prefix_bytes(const PrefixPlan &p, int dh) { return prefix_ml_bytes(p) + (size_t)p.slots() * p.slot_rows * dh * 4; }
+
+}  // namespace lcu

@@ -202,6 +202,25 @@ def test_values_that_are_not_finite_stay_with_their_rows(L):
     assert torch.equal(a.o[1, :4], b.o[1, :4]) and torch.equal(a.o[2], b.o[2])
 
 
+@pytest.mark.parametrize("filth", [math.nan, math.inf])
+def test_values_that_only_later_drafts_see(L, filth):
+    """Drafted tokens share their keys' tiles: what the last one alone sees is not finite, and the others' rows stay as they were."""
+    a, b = (Batch(17, [(20, 4), (16, 3), (49, 2)], 40, 8, 2, 128, 0, 16) for _ in range(2))
+    for seq, slot in ((0, 19), (1, 15), (2, 48)):
+        b.pool[int(b.ids[seq, slot // 16]), 1, :, slot % 16] = filth
+    a.run(L)
+    b.run(L)
+    last = [3, 6, 8]
+    others = [t for t in range(9) if t not in last]
+    assert not b.o[last].isfinite().any()
+    for t in others:
+        assert (a.o[t].double() - b.o[t].double()).abs().max() <= 2.0 ** -10 * a.o[t].abs().max().item()  # (sums in another order)
+    b.pool = a.pool
+    b.o = b.o[others].clone()
+    b.tok_seq, b.ctx, b.q, b.n = b.tok_seq[others], b.ctx[others], b.q[others], len(others)
+    b.check()
+
+
 def test_the_same_answer_twice_and_on_another_stream(L):
     """No atomics: the same bits in every run; two calls at once with workspaces of their own."""
     b = [Batch(15 + i, [(100, 2)] * 9, 3000, 32, 8, 128, 0, 64) for i in range(2)]
