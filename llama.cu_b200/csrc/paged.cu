@@ -30,9 +30,7 @@ struct RowsArgs {
 };
 
 // Where a token goes: false when nothing of it is written (padding, or indices outside what the call names).
-__device__ __forceinline__ bool rw_place(const RowsArgs &a, int t, uint32_t &p, size_t &off) {
-    p = a.pos && a.rot ? a.pos[t] : 0u;
-    if (a.rot && p >= a.n_pos) return false;
+__device__ __forceinline__ bool rw_place(const RowsArgs &a, int t, size_t &off) {
     off = 0;
     if (!a.table) return true;
     const int seq = a.tok_seq[t];
@@ -95,26 +93,23 @@ template <> __device__ __forceinline__ float rw_f<float>(float v) { return v; }
 template <class T> __device__ __forceinline__ T rw_t(float v) { return Act<T>::from_f(v); }
 template <> __device__ __forceinline__ float rw_t<float>(float v) { return v; }
 
-// LPR lanes of a warp hold a row of dh <= 8 LPR values; R rows per lane group, requested before the first is used.
+// LPR lanes of a warp hold a row of dh <= 8 LPR values; R rows per lane group.  Rows, tables and the page's id are requested before any
+// of them is used: three chains of loads side by side.
 template <class T, int LPR, int R>
 __global__ void __launch_bounds__(RW_THREADS) rows_kernel(const RowsArgs a) {
-    constexpr int GROUPS = RW_THREADS / LPR;
-    const int t = blockIdx.x, c = threadIdx.x % LPR, d = 8 * c, total = a.nh + a.nkvh + a.n_v;
-    const int r0 = blockIdx.y * (GROUPS * R) + threadIdx.x / LPR;
-    const bool in = d < a.dh;
+    const int t = blockIdx.x, c = threadIdx.x % LPR, d = 8 * c, total = a.nh + a.nkvh + a.n_v, groups = blockDim.x / LPR;
+    const int r0 = blockIdx.y * (groups * R) + threadIdx.x / LPR;
+    const bool in = d < a.dh, turned = d < a.rot;
+    const uint32_t p = a.rot ? a.pos[t] : 0u;
     Row8<T> x[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-        const int r = r0 + j * GROUPS;
+        const int r = r0 + j * groups;
         if (in && r < total) x[j].load(rw_src<T>(a, t, r) + d);
     }
-    uint32_t p;
-    size_t off;
-    if (!rw_place(a, t, p, off)) return;
     const int half = a.rot >> 1;
     float sn[8], cs[8];  // of the 8 values (halves), or of the 4 pairs
-    const bool turned = d < a.rot;
-    if (turned) {
+    if (turned && p < a.n_pos) {
         const size_t at = (size_t)p * half + (a.halves ? (d < half ? d : d - half) : d >> 1);
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
@@ -124,10 +119,13 @@ __global__ void __launch_bounds__(RW_THREADS) rows_kernel(const RowsArgs a) {
             cs[i] = c4.x; cs[i + 1] = c4.y; cs[i + 2] = c4.z; cs[i + 3] = c4.w;
         }
     }
+    size_t off;
+    const bool placed = rw_place(a, t, off);
+    if (!placed || (a.rot && p >= a.n_pos)) return;
     const int step = half >> 3, partner = a.halves && turned ? (d < half ? c + step : c - step) : c;  // lane of the row that holds the other halves
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-        const int r = r0 + j * GROUPS;
+        const int r = r0 + j * groups;
         const bool is_v = r >= a.nh + a.nkvh;  // (rows past the last take part in the shuffles)
         const void *w = r < a.nh ? a.q_w : a.k_w;
         float f[8];
@@ -181,9 +179,9 @@ template <class T>
 __global__ void __launch_bounds__(RW_THREADS) rows_any_kernel(const RowsArgs a) {
     __shared__ float rows[RW_THREADS / 32][RW_MAX_HEAD];
     const int t = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * (RW_THREADS / 32) + (threadIdx.x >> 5);
-    uint32_t p;
+    const uint32_t p = a.rot ? a.pos[t] : 0u;
     size_t off;
-    if (r >= a.nh + a.nkvh + a.n_v || !rw_place(a, t, p, off)) return;
+    if (r >= a.nh + a.nkvh + a.n_v || (a.rot && p >= a.n_pos) || !rw_place(a, t, off)) return;
     const T *src = rw_src<T>(a, t, r);
     T *dst = rw_dst<T>(a, t, r, off);
     if (r >= a.nh + a.nkvh) {
@@ -217,13 +215,17 @@ __global__ void __launch_bounds__(RW_THREADS) rows_any_kernel(const RowsArgs a) 
 
 template <class T, int LPR>
 static int rows_launch(const RowsArgs &a, int n, cudaStream_t s) {
-    constexpr int GROUPS = RW_THREADS / LPR;
-    const int rows = a.nh + a.nkvh + a.n_v, parts = (rows + GROUPS - 1) / GROUPS;
-    // few tokens: a block per pass over the heads (latency); many: a token's block keeps its tables for several passes
-    if ((long long)n * parts <= 8LL * sm_count() || parts == 1)
-        rows_kernel<T, LPR, 1><<<dim3(n, parts), RW_THREADS, 0, s>>>(a);
-    else
-        rows_kernel<T, LPR, 3><<<dim3(n, (parts + 2) / 3), RW_THREADS, 0, s>>>(a);
+    const int rows = a.nh + a.nkvh + a.n_v;
+    // few tokens: blocks of as many rows as fit, one per lane group (latency); many: a block per token with four rows per lane group, no
+    // larger than its rows (a thread requests 64 bytes at once, and the tables are read once for four rows)
+    constexpr int most = RW_THREADS / LPR;
+    if ((long long)n * ((rows + most - 1) / most) <= 4LL * sm_count()) {
+        rows_kernel<T, LPR, 1><<<dim3(n, (rows + most - 1) / most), RW_THREADS, 0, s>>>(a);
+    } else {
+        const int parts = (rows + 4 * most - 1) / (4 * most), per = (rows + parts - 1) / parts;
+        const int threads = ((per + 3) / 4 * LPR + 31) / 32 * 32;
+        rows_kernel<T, LPR, 4><<<dim3(n, (rows + threads / LPR * 4 - 1) / (threads / LPR * 4)), threads, 0, s>>>(a);
+    }
     LCU_CHECK_CUDA(cudaGetLastError());
     return LCU_OK;
 }

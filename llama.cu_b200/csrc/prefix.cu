@@ -225,16 +225,21 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + 128 * t, to = tmem_o + ((uint32_t)(q * 32) << 16) + DH * t;
         auto load_q = [&](const PfPiece &p) {  // 16 bytes per thread and step, as the 128-byte swizzle has them; zeros behind the last row
             constexpr int CH = DH / 8;
-            const int i = tid - 64 - 128 * t;
-#pragma unroll 4
+            const int i = tid - 64 - 128 * t, c = i % CH;
+            uint4 u[CH];
+#pragma unroll
             for (int k = 0; k < CH; ++k) {
-                const int r = i / CH + k * (128 / CH), c = i % CH, at = 128 * t + r;
-                uint4 u = make_uint4(0, 0, 0, 0);
+                const int at = 128 * t + i / CH + k * (128 / CH);
+                u[k] = make_uint4(0, 0, 0, 0);
                 if (at < p.rows) {
                     const int tok = (p.row0 + at) / group, g = p.row0 + at - tok * group;
-                    u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + (size_t)tok * a.stq + (size_t)(p.hkv * group + g) * a.shq + 8 * c);
+                    u[k] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + (size_t)tok * a.stq + (size_t)(p.hkv * group + g) * a.shq + 8 * c);
                 }
-                *reinterpret_cast<uint4 *>(Qs + t * TILE + (c >> 3) * AT_BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u;
+            }
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+                const int r = i / CH + k * (128 / CH);
+                *reinterpret_cast<uint4 *>(Qs + t * TILE + (c >> 3) * AT_BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[k];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -649,18 +654,47 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
         if (a.prefix_len) {
             const int row = tok * group + g;  // of the KV head
             const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, last = a.plan.last_cta(pair);
-            for (long long c = a.plan.first_cta(pair); c <= last; ++c) {
-                const size_t at = (size_t)(c + pair) * a.plan.slot_rows + row % PF_ROWS;
-                const float2 x = __ldcg(a.part_ml + at);
-                float v[PD];
-                if constexpr (PD == 4) {
-                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at * DH) + lane);
-                    v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
-                } else {
-                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(a.part_o + at * DH) + lane);
-                    v[0] = y.x; v[1] = y.y;
+            // all maxima first, a part per lane, then the parts four at a time: two round trips for up to 32 parts
+            const long long first = a.plan.first_cta(pair);
+            const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS;
+            const int parts_n = (int)(last - first) + 1;
+            float M = p.m;
+            float2 x = make_float2(-INFINITY, 0.f);
+            for (int s0 = 0; s0 < parts_n; s0 += 32) {
+                x = s0 + lane < parts_n ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
+                M = fmaxf(M, warp_max(x.x));
+            }
+            const float f = ow_factor(p.m, M);
+            p.l *= f;
+#pragma unroll
+            for (int i = 0; i < PD; ++i) p.o[i] *= f;
+            for (int s0 = 0; s0 < parts_n; s0 += 32) {
+                if (parts_n > 32) x = s0 + lane < parts_n ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
+                const float g = ow_factor(x.x, M);
+                p.l += warp_sum(x.y * g);
+                const int m = min(32, parts_n - s0);
+#pragma unroll 1
+                for (int s = 0; s < m; s += 4) {
+                    float v[4][PD];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float *src = a.part_o + (at0 + (size_t)(s0 + min(s + i, m - 1)) * a.plan.slot_rows) * DH;
+                        if constexpr (PD == 4) {
+                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(src) + lane);
+                            v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
+                        } else {
+                            const float2 y = __ldcg(reinterpret_cast<const float2 *>(src) + lane);
+                            v[i][0] = y.x; v[i][1] = y.y;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = __shfl_sync(0xffffffffu, g, s + i & 31);
+                        if (s + i < m)
+#pragma unroll
+                            for (int d = 0; d < PD; ++d) p.o[d] = fmaf(v[i][d], w, p.o[d]);
+                    }
                 }
-                add(p, x.x, x.y, v);
             }
         }
         const float inv = p.l == 0.f ? 0.f : 1.f / p.l;

@@ -4,7 +4,7 @@
 
 namespace lcu {
 
-constexpr int VF_THREADS = 512;
+constexpr int VF_THREADS = 256, SM_THREADS = 512;
 constexpr int VF_CLUSTER = 8;
 
 __device__ __forceinline__ void vf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -51,9 +51,9 @@ __device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
 }
 
 template <class T, bool VEC, int EPT>
-__global__ void __launch_bounds__(VF_THREADS) softmax_kernel(const SoftmaxArgs a) {
+__global__ void __launch_bounds__(SM_THREADS) softmax_kernel(const SoftmaxArgs a) {
     constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    __shared__ unsigned long long part[VF_THREADS / 32], xchg[VF_CLUSTER];
+    __shared__ unsigned long long part[SM_THREADS / 32], xchg[VF_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = vf_rank(), size = gridDim.x;
     const int row = blockIdx.y;
@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(VF_THREADS) softmax_kernel(const SoftmaxArgs a
         for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
         if (lane == 0) part[warp] = v;
         __syncthreads();
-        v = part[lane % (VF_THREADS / 32)];
+        v = part[lane % (SM_THREADS / 32)];
 #pragma unroll
-        for (int o = VF_THREADS / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+        for (int o = SM_THREADS / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
         __syncthreads();
         return v;
     };
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(VF_THREADS) softmax_kernel(const SoftmaxArgs a
     auto greater = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
 
     float keep[EPT > 0 ? EPT : V];
-    const size_t first = lo + (size_t)tid * V, step = (size_t)VF_THREADS * V;
+    const size_t first = lo + (size_t)tid * V, step = (size_t)SM_THREADS * V;
     if (t == 0.f) {  // (uniform over the cluster)
         unsigned long long best = 0;
         for (size_t i = first; i < hi; i += step) {
@@ -216,7 +216,7 @@ struct VerifyArgs {
     size_t n, slice, piece;
 };
 
-constexpr int VF_PIECES = 1024;
+constexpr int VF_PIECES = 1024, VF_PIECE = 512;
 
 __device__ __forceinline__ double vf_weight(double p, double q) {
     const double w = p - q;
@@ -226,6 +226,7 @@ __device__ __forceinline__ double vf_weight(double p, double q) {
 template <class T, bool VEC>
 __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) {
     constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    constexpr int AHEAD = VF_PIECE / (32 * V) < 4 ? VF_PIECE / (32 * V) : 4;  // requests of a lane per row before the first value is used
     __shared__ double piece_sum[VF_PIECES], total[VF_CLUSTER];
     __shared__ int s_n;
     __shared__ double s_thr;
@@ -275,45 +276,64 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     const size_t lo = (size_t)rank * a.slice < a.n ? (size_t)rank * a.slice : a.n, hi = lo + a.slice < a.n ? lo + a.slice : a.n;
     const int pieces = (int)((hi - lo + a.piece - 1) / a.piece);
 
-    // weights of V values from i on (i < hi); minus: what the draft gave comes off
-    auto weights = [&](size_t i, bool minus, double *w) {
-        float p[V], q[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) p[e] = q[e] = 0.f;
-        const bool sub = minus && Q;
-        if (VEC && i + V <= hi) {
-            const uint4 up = *reinterpret_cast<const uint4 *>(P + i), uq = sub ? *reinterpret_cast<const uint4 *>(Q + i) : make_uint4(0, 0, 0, 0);
-            const uint32_t wp[4] = {up.x, up.y, up.z, up.w}, wq[4] = {uq.x, uq.y, uq.z, uq.w};
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) p[e] = __uint_as_float(wp[e]), q[e] = __uint_as_float(wq[e]);
+    // V values of a row from i on, zeros behind the slice; as 16 bytes where rows are
+    struct Raw {
+        uint32_t u[VEC ? 4 : 1];
+    };
+    auto read = [&](const T *row, size_t i) {
+        Raw r;
+        if constexpr (VEC) {
+            if (i + V <= hi) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(row + i);
+                r.u[0] = q.x; r.u[1] = q.y; r.u[2] = q.z; r.u[3] = q.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    const float2 f = Act<T>::to_f2(wp[e / 2]), g = Act<T>::to_f2(wq[e / 2]);
-                    p[e] = f.x; p[e + 1] = f.y; q[e] = g.x; q[e + 1] = g.y;
-                }
+                for (int e = 0; e < 4; ++e) r.u[e] = 0u;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (i + e < hi) {
+                        if constexpr (sizeof(T) == 4) r.u[e] = __float_as_uint(row[i + e]);
+                        else r.u[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[i + e] << (16 * (e & 1));
+                    }
             }
         } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (i + e < hi) {
-                    p[e] = vf_f<T>(P[i + e]);
-                    if (sub) q[e] = vf_f<T>(Q[i + e]);
-                }
+            r.u[0] = i < hi ? __float_as_uint(vf_f<T>(row[i])) : 0u;
         }
+        return r;
+    };
+    auto value = [&](const Raw &r, int e) {
+        if constexpr (!VEC || sizeof(T) == 4) return __uint_as_float(r.u[e]);
+        else {
+            const float2 f = Act<T>::to_f2(r.u[e / 2]);
+            return e & 1 ? f.y : f.x;
+        }
+    };
+    // their weights; minus: what the draft gave comes off
+    auto weights = [&](size_t i, bool minus, const Raw &p, const Raw &q, double *w) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[e] = vf_weight((double)p[e], minus && !Q && (long long)(i + e) == x_held ? 1. : (double)q[e]);
+        for (int e = 0; e < V; ++e) {
+            const double off = minus ? (Q ? (double)value(q, e) : (long long)(i + e) == x_held ? 1. : 0.) : 0.;
+            w[e] = vf_weight((double)value(p, e), off);
+        }
     };
     auto sums = [&](bool minus) {  // of the pieces, a warp each; the CTA's total goes to everyone
         for (int j = warp; j < pieces; j += VF_THREADS / 32) {
             const size_t p0 = lo + (size_t)j * a.piece, p1 = p0 + a.piece < hi ? p0 + a.piece : hi;
             double s = 0.;
-            for (size_t i = p0 + (size_t)lane * V; i < p1; i += 32 * V) {
-                double w[V];
-                weights(i, minus, w);
+            for (size_t i = p0 + (size_t)lane * V; i < p1; i += AHEAD * 32 * V) {
+                Raw p[AHEAD], q[AHEAD];
 #pragma unroll
-                for (int e = 0; e < V; ++e) s += w[e];
+                for (int h = 0; h < AHEAD; ++h) {
+                    p[h] = read(P, i + h * 32 * V);
+                    if (minus && Q) q[h] = read(Q, i + h * 32 * V);
+                }
+#pragma unroll
+                for (int h = 0; h < AHEAD; ++h) {
+                    double w[V];
+                    weights(i + h * 32 * V, minus, p[h], q[h], w);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s += w[e];
+                }
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -377,7 +397,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
         double w[V], mine = 0.;
 #pragma unroll
         for (int e = 0; e < V; ++e) w[e] = 0.;
-        if (i < p1) weights(i, minus, w);
+        if (i < p1) weights(i, minus, read(P, i), minus && Q ? read(Q, i) : Raw{}, w);
 #pragma unroll
         for (int e = 0; e < V; ++e) mine += w[e];
         double upto = mine;
@@ -407,10 +427,10 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
 // ------------------------------------------------------------------ host side
 
 template <class... KArgs>
-static int vf_launch(void (*kernel)(KArgs...), int cluster, int rows, cudaStream_t s, KArgs... args) {
+static int vf_launch(void (*kernel)(KArgs...), int threads, int cluster, int rows, cudaStream_t s, KArgs... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster, rows);
-    cfg.blockDim = dim3(VF_THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -426,17 +446,17 @@ template <class T, bool VEC>
 static int softmax_launch(SoftmaxArgs a, int rows, cudaStream_t s) {
     // CTAs of a row: as many as give every thread 16 values or more
     int c = 1;
-    while (c < VF_CLUSTER && a.n > (size_t)c * VF_THREADS * 16) c *= 2;
+    while (c < VF_CLUSTER && a.n > (size_t)c * SM_THREADS * 16) c *= 2;
     a.slice = ((a.n + c - 1) / c + 7) / 8 * 8;
-    const size_t per = (a.slice + VF_THREADS - 1) / VF_THREADS;
+    const size_t per = (a.slice + SM_THREADS - 1) / SM_THREADS;
     for (int r0 = 0; r0 < rows; r0 += 65535) {
         SoftmaxArgs b = a;
         b.probs += (size_t)r0 * a.stride_p;
         b.logits = reinterpret_cast<const T *>(a.logits) + (size_t)r0 * a.stride_l;
         if (b.temperature) b.temperature += r0;
         const int m = rows - r0 < 65535 ? rows - r0 : 65535;
-        const int rc = per <= 8 ? vf_launch(softmax_kernel<T, VEC, 8>, c, m, s, (const SoftmaxArgs)b) : per <= 16 ? vf_launch(softmax_kernel<T, VEC, 16>, c, m, s, (const SoftmaxArgs)b)
-                     : per <= 32 ? vf_launch(softmax_kernel<T, VEC, 32>, c, m, s, (const SoftmaxArgs)b) : vf_launch(softmax_kernel<T, VEC, 0>, c, m, s, (const SoftmaxArgs)b);
+        const int rc = per <= 8 ? vf_launch(softmax_kernel<T, VEC, 8>, SM_THREADS, c, m, s, (const SoftmaxArgs)b) : per <= 16 ? vf_launch(softmax_kernel<T, VEC, 16>, SM_THREADS, c, m, s, (const SoftmaxArgs)b)
+                     : per <= 32 ? vf_launch(softmax_kernel<T, VEC, 32>, SM_THREADS, c, m, s, (const SoftmaxArgs)b) : vf_launch(softmax_kernel<T, VEC, 0>, SM_THREADS, c, m, s, (const SoftmaxArgs)b);
         if (rc) return rc;
     }
     return LCU_OK;
@@ -452,8 +472,8 @@ template <class T>
 static int verify_t(VerifyArgs a, int n_seq, cudaStream_t s) {
     int c = 1;
     while (c < VF_CLUSTER && a.n > (size_t)c * 4096) c *= 2;
-    a.piece = 512;
-    a.slice = ((a.n + c - 1) / c + 511) / 512 * 512;
+    a.piece = VF_PIECE;
+    a.slice = ((a.n + c - 1) / c + VF_PIECE - 1) / VF_PIECE * VF_PIECE;
     while (a.slice / a.piece > VF_PIECES) {
         a.piece *= 2;
         a.slice = ((a.n + c - 1) / c + a.piece - 1) / a.piece * a.piece;
@@ -470,7 +490,7 @@ static int verify_t(VerifyArgs a, int n_seq, cudaStream_t s) {
         if (a.n_drafted) v.n_drafted += b0;
         v.randoms += b0 * (k + 1);
         const int m = n_seq - b0 < 65535 ? n_seq - b0 : 65535;
-        const int rc = vec ? vf_launch(verify_kernel<T, true>, c, m, s, (const VerifyArgs)v) : vf_launch(verify_kernel<T, false>, c, m, s, (const VerifyArgs)v);
+        const int rc = vec ? vf_launch(verify_kernel<T, true>, VF_THREADS, c, m, s, (const VerifyArgs)v) : vf_launch(verify_kernel<T, false>, VF_THREADS, c, m, s, (const VerifyArgs)v);
         if (rc) return rc;
     }
     return LCU_OK;
