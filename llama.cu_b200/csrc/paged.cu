@@ -4,15 +4,20 @@
 //   y = x w / sqrt(mean(x^2) + eps)                   per head, where there are weights
 //   (a, b) -> (a cos - b sin, a sin + b cos)          of the first rot_dims values, pairs (2 i, 2 i + 1) or (i, i + rot_dims / 2)
 //
-// all in 32 bits with one rounding at the end.  Bound by HBM: every row is read once and written once.  A row of dh values is held by
-// dh / 8 lanes, 8 values each (the partner of a half-split pair is a shuffle away), and a thread keeps the sin and cos of its values
-// for every row of the token that it takes: a block is a token, so the tables are read once per thread and not once per row.
+// all in 32 bits with one rounding at the end.  Every row is read once and written once, so HBM is the floor; what has to be kept down
+// on the way there is instructions and waits.  heads_kernel: a row is held by dh / 16 lanes, each with 8 values of the lower half and the
+// 8 that stand dh / 2 behind them, so that the pairs of either kind meet in one thread; lanes stay with their head from token to token
+// and request the next token's row while they work on one.  rows_kernel takes what heads_kernel cannot (halves of
+// a part of the head), rows_any_kernel the rest (sizes, strides or addresses that are no multiples of 16 bytes).
 #include "paged.cuh"
+
+#include <mutex>
 
 namespace lcu {
 
 constexpr int RW_THREADS = 256;
 constexpr int RW_MAX_HEAD = 256;
+constexpr int HK_THREADS = 128, HK_STAGES = 4, HK_BLOCKS = 5;  // (4 blocks of 16-bit rows on an SM 3 % slower, 6 spill registers and are a third slower)
 
 struct RowsArgs {
     const void *q, *k, *v;
@@ -29,16 +34,30 @@ struct RowsArgs {
     int w_f32, rot, halves, nh, nkvh, n_v, dh;  // n_v: value rows of a token (0 without a cache)
 };
 
-// Where a token goes: false when nothing of it is written (padding, or indices outside what the call names).
-__device__ __forceinline__ bool rw_place(const RowsArgs &a, int t, size_t &off) {
+// What is read of a token ahead of its rows, and where it goes (in steps: the page id is a load behind the others).
+struct RowsToken {
+    uint32_t pos, slot;
+    int seq, page;
+};
+__device__ __forceinline__ void rw_token(const RowsArgs &a, int t, RowsToken &k) {
+    k.pos = a.rot ? a.pos[t] : 0u;
+    k.seq = a.table ? a.tok_seq[t] : 0;
+    k.slot = a.table ? a.slot[t] : 0u;
+}
+// false when nothing of it is written: padding, or indices outside what the call names
+__device__ __forceinline__ bool rw_page(const RowsArgs &a, RowsToken &k) {
+    k.page = 0;
+    if (a.rot && k.pos >= a.n_pos) return false;
+    if (!a.table) return true;
+    if (k.seq < 0 || k.seq >= a.n_seq || (k.slot >> a.page_shift) >= (uint32_t)a.table_stride) return false;
+    k.page = a.table[(size_t)k.seq * a.table_stride + (k.slot >> a.page_shift)];
+    return true;
+}
+__device__ __forceinline__ bool rw_place(const RowsArgs &a, const RowsToken &k, size_t &off) {
     off = 0;
     if (!a.table) return true;
-    const int seq = a.tok_seq[t];
-    const uint32_t slot = a.slot[t];
-    if (seq < 0 || seq >= a.n_seq || (slot >> a.page_shift) >= (uint32_t)a.table_stride) return false;
-    const int page = a.table[(size_t)seq * a.table_stride + (slot >> a.page_shift)];
-    if (page < 0 || page >= a.pages.n_pages) return false;
-    off = (size_t)page * a.pages.stride_page + (size_t)(slot & ((1u << a.page_shift) - 1)) * a.pages.stride_tok;
+    if (k.page < 0 || k.page >= a.pages.n_pages) return false;
+    off = (size_t)k.page * a.pages.stride_page + (size_t)(k.slot & ((1u << a.page_shift) - 1)) * a.pages.stride_tok;
     return true;
 }
 
@@ -63,6 +82,7 @@ template <class T> __device__ __forceinline__ T *rw_dst(const RowsArgs &a, int t
 template <class T> struct Row8 {
     uint4 u;
     __device__ __forceinline__ void load(const T *p) { u = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void load(const uint4 *p, int) { u = *p; }  // pieces of 16 bytes, `step` of them apart
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = u; }
     __device__ __forceinline__ void get(float *f) const {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -80,6 +100,11 @@ template <class T> struct Row8 {
 template <> struct Row8<float> {
     float4 x, y;
     __device__ __forceinline__ void load(const float *p) { x = reinterpret_cast<const float4 *>(p)[0]; y = reinterpret_cast<const float4 *>(p)[1]; }
+    __device__ __forceinline__ void load(const uint4 *p, int step) {
+        const uint4 a = p[0], b = p[step];
+        x = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
+        y = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
+    }
     __device__ __forceinline__ void store(float *p) const { reinterpret_cast<float4 *>(p)[0] = x; reinterpret_cast<float4 *>(p)[1] = y; }
     __device__ __forceinline__ void get(float *f) const {
         f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
@@ -93,6 +118,171 @@ template <> __device__ __forceinline__ float rw_f<float>(float v) { return v; }
 template <class T> __device__ __forceinline__ T rw_t(float v) { return Act<T>::from_f(v); }
 template <> __device__ __forceinline__ float rw_t<float>(float v) { return v; }
 
+__device__ __forceinline__ unsigned long long rw_pair(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 rw_unpair(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long rw_fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ unsigned long long rw_mul2(unsigned long long x, unsigned long long y) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// LPR lanes hold a row of dh <= 16 LPR values, each 8 from 8 c and 8 from dh / 2 + 8 c on.  HALVES: rot == dh, pairs (i, i + dh / 2).
+// Otherwise pairs (2 i, 2 i + 1).  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every gridDim.x-th token.
+template <class T, int LPR, bool HALVES, bool WF>
+__global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) heads_kernel(const RowsArgs a, int n, int rows_per) {
+    const int c = threadIdx.x % LPR, local = threadIdx.x / LPR, r = blockIdx.y * rows_per + local, total = a.nh + a.nkvh + a.n_v;
+    const int lower = a.dh / 2, d = 8 * c;
+    const bool in = d < lower && local < rows_per && r < total, is_q = r < a.nh, is_v = r >= a.nh + a.nkvh;
+    // where this lane reads and writes for token 0; from token to token, or by the token's place in the pages
+    const T *src = in ? rw_src<T>(a, 0, r) + d : nullptr;
+    T *dst = in ? rw_dst<T>(a, 0, r, 0) + d : nullptr;
+    const int src_step = is_q ? a.stq : is_v ? a.stv : a.stk, dst_step = is_q ? a.stqo : a.stko;
+    const bool paged = a.table && !is_q;
+    const void *w = in && !is_v ? (is_q ? a.q_w : a.k_w) : nullptr;
+    const bool any_norm = __any_sync(0xffffffffu, w != nullptr);  // of the warp's rows
+    Row8<T> g0, g1;                                               // this head's weights (f32 ones are read from L1 each time)
+    if (w && !WF) {
+        g0.load(reinterpret_cast<const T *>(w) + d);
+        g1.load(reinterpret_cast<const T *>(w) + lower + d);
+    }
+    const int half = a.rot >> 1;
+    const bool turn0 = in && !is_v && d < a.rot, turn1 = in && !is_v && lower + d < a.rot;
+    const int at0 = HALVES ? d : d >> 1, at1 = HALVES ? d + 4 : (lower + d) >> 1;  // of a row of the tables
+    const float inv_dh = 1.f / (float)a.dh;
+    // Rows of the next tokens on their way into shared memory, each thread's own: [stage][16-byte piece][thread].
+    constexpr int PIECES = (int)sizeof(T), HALF = PIECES / 2;  // 16 values
+    __shared__ uint4 ring[HK_STAGES][PIECES][HK_THREADS];
+    const int stride = gridDim.x;
+    auto request = [&](int stage, long long tok) {
+        if (in && tok < n) {
+            const T *p = src + (size_t)tok * src_step;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const T *q = p + (i < HALF ? 0 : lower) + i % HALF * (16 / (int)sizeof(T));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&ring[stage][i][threadIdx.x])), "l"(q) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int t = blockIdx.x, stage = 0;
+    RowsToken cur, ahead;
+    rw_token(a, t, cur);
+#pragma unroll
+    for (int i = 0; i < HK_STAGES - 1; ++i) request(i, t + (long long)i * stride);
+    if (t + stride < n) rw_token(a, t + stride, ahead);
+    bool go = rw_page(a, cur);
+    for (; t < n; t += stride, stage = stage + 1 == HK_STAGES ? 0 : stage + 1) {
+        // HALVES: sin and cos of the 8 pairs; else of 4 pairs of either half
+        float4 sn0, sn1, cs0, cs1;
+        const float *sn_row = a.sin_t + (size_t)cur.pos * half, *cs_row = a.cos_t + (size_t)cur.pos * half;
+        if (go && turn0) {
+            sn0 = *reinterpret_cast<const float4 *>(sn_row + at0);
+            cs0 = *reinterpret_cast<const float4 *>(cs_row + at0);
+        }
+        if (go && turn1) {
+            sn1 = *reinterpret_cast<const float4 *>(sn_row + at1);
+            cs1 = *reinterpret_cast<const float4 *>(cs_row + at1);
+        }
+        const RowsToken now = cur;
+        const bool here = go;
+        go = false;
+        request(stage == 0 ? HK_STAGES - 1 : stage - 1, t + (HK_STAGES - 1) * (long long)stride);
+        if (t + stride < n) {
+            cur = ahead;
+            go = rw_page(a, cur);
+            if (t + 2 * (long long)stride < n) rw_token(a, t + 2 * stride, ahead);
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(HK_STAGES - 1) : "memory");  // this thread's own copies: nobody else is waited for
+        size_t off;
+        if (!here || !rw_place(a, now, off)) continue;  // (of the whole block)
+        Row8<T> x0, x1;
+        x0.load(reinterpret_cast<const uint4 *>(&ring[stage][0][threadIdx.x]), HK_THREADS);
+        x1.load(reinterpret_cast<const uint4 *>(&ring[stage][HALF][threadIdx.x]), HK_THREADS);
+        if (!is_v || any_norm) {                        // (lanes of values go along with others' shuffles)
+            float u[8], v[8];
+            x0.get(u);
+            x1.get(v);
+            float k = 1.f;
+            if (any_norm) {
+                unsigned long long s2 = rw_mul2(rw_pair(u[0], u[1]), rw_pair(u[0], u[1]));
+#pragma unroll
+                for (int i = 1; i < 4; ++i) s2 = rw_fma2(rw_pair(u[2 * i], u[2 * i + 1]), rw_pair(u[2 * i], u[2 * i + 1]), s2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s2 = rw_fma2(rw_pair(v[2 * i], v[2 * i + 1]), rw_pair(v[2 * i], v[2 * i + 1]), s2);
+                const float2 s = rw_unpair(s2);
+                float ss = in ? s.x + s.y : 0.f;
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (w) {
+                    k = rsqrtf(ss * inv_dh + a.eps);
+                    float g[8], h[8];
+                    if (WF) {
+                        Row8<float> y0, y1;
+                        y0.load(reinterpret_cast<const float *>(w) + d);
+                        y1.load(reinterpret_cast<const float *>(w) + lower + d);
+                        y0.get(g);
+                        y1.get(h);
+                    } else {
+                        g0.get(g);
+                        g1.get(h);
+                    }
+                    const unsigned long long k2 = rw_pair(k, k);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const float2 x = rw_unpair(rw_mul2(rw_mul2(rw_pair(u[i], u[i + 1]), k2), rw_pair(g[i], g[i + 1])));
+                        const float2 y = rw_unpair(rw_mul2(rw_mul2(rw_pair(v[i], v[i + 1]), k2), rw_pair(h[i], h[i + 1])));
+                        u[i] = x.x; u[i + 1] = x.y; v[i] = y.x; v[i + 1] = y.y;
+                    }
+                }
+            }
+            if (HALVES) {
+                if (turn0) {
+                    const float sn[8] = {sn0.x, sn0.y, sn0.z, sn0.w, sn1.x, sn1.y, sn1.z, sn1.w}, cs[8] = {cs0.x, cs0.y, cs0.z, cs0.w, cs1.x, cs1.y, cs1.z, cs1.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float x = u[i], y = v[i];
+                        u[i] = x * cs[i] - y * sn[i];
+                        v[i] = x * sn[i] + y * cs[i];
+                    }
+                }
+            } else {
+                auto turn = [](float *f, const float4 &sn, const float4 &cs) {
+                    const float s[4] = {sn.x, sn.y, sn.z, sn.w}, c[4] = {cs.x, cs.y, cs.z, cs.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = f[2 * i], y = f[2 * i + 1];
+                        f[2 * i] = x * c[i] - y * s[i];
+                        f[2 * i + 1] = x * s[i] + y * c[i];
+                    }
+                };
+                if (turn0) turn(u, sn0, cs0);
+                if (turn1) turn(v, sn1, cs1);
+            }
+            if (!is_v) {
+                x0.set(u);
+                x1.set(v);
+            }
+        }
+        if (!in) continue;
+        T *p = dst + (paged ? off : (size_t)t * dst_step);
+        x0.store(p);
+        x1.store(p + lower);
+    }
+}
+
 // LPR lanes of a warp hold a row of dh <= 8 LPR values; R rows per lane group.  Rows, tables and the page's id are requested before any
 // of them is used: three chains of loads side by side.
 template <class T, int LPR, int R>
@@ -100,7 +290,9 @@ __global__ void __launch_bounds__(RW_THREADS) rows_kernel(const RowsArgs a) {
     const int t = blockIdx.x, c = threadIdx.x % LPR, d = 8 * c, total = a.nh + a.nkvh + a.n_v, groups = blockDim.x / LPR;
     const int r0 = blockIdx.y * (groups * R) + threadIdx.x / LPR;
     const bool in = d < a.dh, turned = d < a.rot;
-    const uint32_t p = a.rot ? a.pos[t] : 0u;
+    RowsToken k;
+    rw_token(a, t, k);
+    const uint32_t p = k.pos;
     Row8<T> x[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -120,8 +312,7 @@ __global__ void __launch_bounds__(RW_THREADS) rows_kernel(const RowsArgs a) {
         }
     }
     size_t off;
-    const bool placed = rw_place(a, t, off);
-    if (!placed || (a.rot && p >= a.n_pos)) return;
+    if (!rw_page(a, k) || !rw_place(a, k, off)) return;
     const int step = half >> 3, partner = a.halves && turned ? (d < half ? c + step : c - step) : c;  // lane of the row that holds the other halves
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -179,9 +370,11 @@ template <class T>
 __global__ void __launch_bounds__(RW_THREADS) rows_any_kernel(const RowsArgs a) {
     __shared__ float rows[RW_THREADS / 32][RW_MAX_HEAD];
     const int t = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * (RW_THREADS / 32) + (threadIdx.x >> 5);
-    const uint32_t p = a.rot ? a.pos[t] : 0u;
+    RowsToken k;
+    rw_token(a, t, k);
+    const uint32_t p = k.pos;
     size_t off;
-    if (r >= a.nh + a.nkvh + a.n_v || (a.rot && p >= a.n_pos) || !rw_place(a, t, off)) return;
+    if (r >= a.nh + a.nkvh + a.n_v || !rw_page(a, k) || !rw_place(a, k, off)) return;
     const T *src = rw_src<T>(a, t, r);
     T *dst = rw_dst<T>(a, t, r, off);
     if (r >= a.nh + a.nkvh) {
@@ -215,9 +408,9 @@ __global__ void __launch_bounds__(RW_THREADS) rows_any_kernel(const RowsArgs a) 
 
 template <class T, int LPR>
 static int rows_launch(const RowsArgs &a, int n, cudaStream_t s) {
-    const int rows = a.nh + a.nkvh + a.n_v;
     // few tokens: blocks of as many rows as fit, one per lane group (latency); many: a block per token with four rows per lane group, no
     // larger than its rows (a thread requests 64 bytes at once, and the tables are read once for four rows)
+    const int rows = a.nh + a.nkvh + a.n_v;
     constexpr int most = RW_THREADS / LPR;
     if ((long long)n * ((rows + most - 1) / most) <= 4LL * sm_count()) {
         rows_kernel<T, LPR, 1><<<dim3(n, (rows + most - 1) / most), RW_THREADS, 0, s>>>(a);
@@ -230,6 +423,30 @@ static int rows_launch(const RowsArgs &a, int n, cudaStream_t s) {
     return LCU_OK;
 }
 
+template <class T, int LPR, bool HALVES, bool WF>
+static int heads_launch(const RowsArgs &a, int n, cudaStream_t s) {
+    // blocks of up to 128 threads with an even part of a token's rows; as many as run at once
+    const int rows = a.nh + a.nkvh + a.n_v, parts = (rows * LPR + HK_THREADS - 1) / HK_THREADS, per = (rows + parts - 1) / parts, threads = (per * LPR + 31) / 32 * 32;
+    static std::mutex mu;
+    static int resident[HK_THREADS / 32 + 1] = {};  // blocks of so many warps that an SM holds
+    int blocks;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        int &have = resident[threads / 32];
+        if (!have) LCU_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&have, heads_kernel<T, LPR, HALVES, WF>, threads, 0));
+        blocks = have * sm_count() / parts;
+    }
+    heads_kernel<T, LPR, HALVES, WF><<<dim3(n < blocks || blocks < 1 ? n : blocks, parts), threads, 0, s>>>(a, n, per);
+    LCU_CHECK_CUDA(cudaGetLastError());
+    return LCU_OK;
+}
+template <class T, int LPR>
+static int heads_form(const RowsArgs &a, int n, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (a.w_f32) return a.halves ? heads_launch<T, LPR, true, true>(a, n, s) : heads_launch<T, LPR, false, true>(a, n, s);
+    return a.halves ? heads_launch<T, LPR, true, false>(a, n, s) : heads_launch<T, LPR, false, false>(a, n, s);
+}
+
 template <class T>
 static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
     if (!vec) {
@@ -237,6 +454,10 @@ static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
         rows_any_kernel<T><<<dim3(n, (rows + per - 1) / per), RW_THREADS, 0, s>>>(a);
         LCU_CHECK_CUDA(cudaGetLastError());
         return LCU_OK;
+    }
+    if (a.dh % 16 == 0 && (!a.halves || a.rot == 0 || a.rot == a.dh)) {
+        const int lanes = a.dh / 16;
+        return lanes <= 2 ? heads_form<T, 2>(a, n, s) : lanes <= 4 ? heads_form<T, 4>(a, n, s) : lanes <= 8 ? heads_form<T, 8>(a, n, s) : heads_form<T, 16>(a, n, s);
     }
     const int lanes = a.dh / 8;
     return lanes <= 4 ? rows_launch<T, 4>(a, n, s) : lanes <= 8 ? rows_launch<T, 8>(a, n, s) : lanes <= 16 ? rows_launch<T, 16>(a, n, s) : rows_launch<T, 32>(a, n, s);

@@ -9,13 +9,15 @@
 //    a KV head fill tiles of 256 rows, so the prefix is read once per 256 rows instead of once per token; the roles, tensor memory and
 //    arithmetic are those of attention_tc.cu.  The units (KV head, row tile, key tile) are dealt to one CTA per SM in equal
 //    contiguous ranges; a CTA leaves one partial result per (KV head, row tile) that it meets.
-//  - own_kernel: each token's own slots, then the sum of all parts.  A CTA owns a KV head and up to 16 query rows of one sequence's
-//    consecutive tokens (drafted tokens share their keys); its four warps take 16 keys each in turns, with a softmax of their own
-//    and both products in registers (mma.sync), and meet once at the end.  It is launched as a programmatic dependent: own slots are worked
-//    on while the prefix runs, and only the sum waits for it.
+//  - own_kernel: each token's own slots.  A CTA owns a KV head and up to 16 query rows of one sequence's consecutive tokens (drafted tokens
+//    share their keys); its two warps take 16 keys each in turns, with a softmax of their own and both products in registers (mma.sync),
+//    and meet once at the end.  It is launched as a programmatic dependent and fits on an SM beside a block of the prefix, under whose
+//    exponentials it loads.
+//  - The sum of all parts: at the end of own_kernel where its blocks are few, else in own_sum_kernel.
 //
-// f32 scores and softmax, weights rounded to the activation type ahead of the second product (its operands are 16-bit; the sums are
-// taken over the rounded weights, so the rounding does not shift the whole row), one rounding of the output.
+// f32 scores and softmax, sums in f32 over the weights as they are, weights rounded to the activation type ahead of the second product (its
+// operands are 16-bit), one rounding of the output.  (Sums over the rounded weights, as attention.cu takes them, are no closer to the
+// softmax where many weights count and cost 4 % of the prefix in conversions; a weight that stands alone is 1 and is not rounded.)
 #include "attention_tc.cuh"
 #include "paged.cuh"
 #include "prefix_plan.hpp"
@@ -33,8 +35,9 @@ struct PrefixArgs {
     int table_stride, n_seq, page_shift, n, nh, nkvh;
     float scale2;  // scores in powers of two
     PrefixPlan plan;
-    float2 *part_ml;  // [slot][row]
-    float *part_o;    // [slot][row][dh]
+    float2 *part_ml;  // [slot][row], then own parts [part][KV head][row]
+    float *part_o;    // ... [dh]
+    size_t own_row;   // where the latter begin
 };
 
 // ------------------------------------------------------------------ the prefix
@@ -44,7 +47,7 @@ constexpr int PF_MAX_STAGES = 4;
 
 struct PfShared {
     unsigned long long k_full[PF_MAX_STAGES], k_empty[PF_MAX_STAGES], v_full[PF_MAX_STAGES], v_empty[PF_MAX_STAGES];
-    unsigned long long q_full[2], s_full[2], p_ready[2], o_done[2], drain;
+    unsigned long long q_full[2], s_full[2], p_ready[2][2], pv_done[2], drain;
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -56,6 +59,23 @@ __device__ __forceinline__ void pf_tma_4d(uint32_t dst, const CUtensorMap *map, 
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
                  " @e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n}"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+// four products of K = 16, weights in tensor memory (8 columns each), values in shared memory (2 KB each): one election for all
+__device__ __forceinline__ void pf_mma_ts4(uint32_t d, uint32_t w, uint64_t v, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred e, p, q;\n .reg .b32 a;\n .reg .b64 b;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 q, 0, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n add.u32 a, %1, 8;\n add.u64 b, %2, 128;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n add.u32 a, %1, 16;\n add.u64 b, %2, 256;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n add.u32 a, %1, 24;\n add.u64 b, %2, 384;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n}"
+                 ::"r"(d), "r"(w), "l"(v), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pf_st8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void pf_arrive(uint32_t bar, int lane) {  // of a warp, behind its accesses to tensor or shared memory
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void pf_st32(float *p, const uint32_t *r) {  // 32 bytes, 16-byte aligned
     reinterpret_cast<uint4 *>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
@@ -108,8 +128,9 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         for (int t = 0; t < 2; ++t) {
             tc_mbar_init(tc_smem(&sh->q_full[t]), 4);
             tc_mbar_init(tc_smem(&sh->s_full[t]), 1);
-            tc_mbar_init(tc_smem(&sh->p_ready[t]), 4);
-            tc_mbar_init(tc_smem(&sh->o_done[t]), 1);
+            tc_mbar_init(tc_smem(&sh->p_ready[t][0]), 4);
+            tc_mbar_init(tc_smem(&sh->p_ready[t][1]), 4);
+            tc_mbar_init(tc_smem(&sh->pv_done[t]), 1);
         }
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -170,7 +191,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         const uint32_t id_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
         const uint64_t q0 = tc_desc(tc_smem(Qs)), k0 = tc_desc(tc_smem(Ks)), v0 = at_desc_mn(tc_smem(Vs));
         const uint32_t kf = tc_smem(&sh->k_full[0]), ke = tc_smem(&sh->k_empty[0]), vf = tc_smem(&sh->v_full[0]), ve = tc_smem(&sh->v_empty[0]);
-        const uint32_t sf = tc_smem(&sh->s_full[0]), pr = tc_smem(&sh->p_ready[0]), od = tc_smem(&sh->o_done[0]), qf = tc_smem(&sh->q_full[0]);
+        const uint32_t sf = tc_smem(&sh->s_full[0]), pr = tc_smem(&sh->p_ready[0][0]), pd = tc_smem(&sh->pv_done[0]), qf = tc_smem(&sh->q_full[0]);
         auto scores = [&](int t, int slot) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -178,7 +199,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
             tc_warp_commit(sf + 8 * t);
         };
         int slot = 0;
-        uint32_t phase = 0, p_phase = 0, q_phase = 0;  // bit t of the last two: tile t's
+        uint32_t phase = 0, p_phase = 0, q_phase = 0, seen = 0;  // bit t of the last three: tile t's; whether it has had products
         bool ok = true;
         for (PfPiece p = pf_piece(a.plan, u0, u1); ok && p.unit < u1; p = pf_next(a.plan, p)) {
             const int nt = p.two ? 2 : 1;
@@ -187,8 +208,11 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                 q_phase ^= 1u << t;
             }
             ok = ok && tc_warp_wait(kf + 8 * slot, phase, &sh->abort_flag);
+            for (int t = 0; t < nt && ok; ++t)
+                if (seen >> t & 1u) ok = tc_warp_wait(pd + 8 * t, (p_phase >> t & 1u) ^ 1u, &sh->abort_flag);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            seen |= nt == 2 ? 3u : 1u;
             for (int t = 0; t < nt; ++t) scores(t, slot);
             tc_warp_commit(ke + 8 * slot);
             for (int j = p.j0; j < p.j1 && ok; ++j) {
@@ -198,20 +222,25 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                 ok = tc_warp_wait(vf + 8 * slot, phase, &sh->abort_flag);
                 if (ok && more) ok = tc_warp_wait(kf + 8 * next, next_phase, &sh->abort_flag);
                 for (int t = 0; t < nt && ok; ++t) {
-                    ok = tc_warp_wait(pr + 8 * t, p_phase >> t & 1u, &sh->abort_flag);
-                    p_phase ^= 1u << t;
+                    for (int h = 0; h < 2 && ok; ++h) {  // weights of 64 positions at a time
+                        ok = tc_warp_wait(pr + 16 * t + 8 * h, p_phase >> t & 1u, &sh->abort_flag);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        pf_mma_ts4(tmem_o + DH * t, tmem + 128 * t + 32 * h, v0 + (uint64_t)((slot * TILE + h * 8192) >> 4), id_o, j > p.j0 || h > 0);
+                    }
                     if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)  // 16 positions: 8 columns of weights, 2 KB of the V tile
-                        at_mma_ts(tmem_o + DH * t, tmem + 128 * t + 8 * k, v0 + (uint64_t)((slot * TILE + k * 2048) >> 4), id_o, j > p.j0 || k > 0);
+                    tc_warp_commit(pd + 8 * t);
                     if (t == nt - 1) tc_warp_commit(ve + 8 * slot);
                     if (more) {
+                        // The next scores go over the columns of these weights.  Products of unlike shapes or accumulators are not ordered
+                        // among themselves, so the ones that read the weights have to have ended (1 % of the time).
+                        ok = tc_warp_wait(pd + 8 * t, p_phase >> t & 1u, &sh->abort_flag);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         scores(t, next);
                         if (t == nt - 1) tc_warp_commit(ke + 8 * next);
-                    } else {
-                        tc_warp_commit(od + 8 * t);
                     }
+                    p_phase ^= 1u << t;
                 }
                 slot = next;
                 phase = next_phase;
@@ -242,17 +271,16 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                 *reinterpret_cast<uint4 *>(Qs + t * TILE + (c >> 3) * AT_BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[k];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(&sh->q_full[t])) : "memory");
+            pf_arrive(tc_smem(&sh->q_full[t]), lane);
         };
         auto bad_pages = [&](int tile) {  // bit i: page i of the tile names no page
             const int i = tile * ppt + lane;
             const int id = lane < ppt && i < n_prefix_pages ? a.prefix_table[i] : 0;
             return __ballot_sync(0xffffffffu, id < 0 || id >= a.pages.n_pages);
         };
+        const uint32_t pr = tc_smem(&sh->p_ready[t][0]);
         int it = 0;          // units of the CTA so far
         uint32_t mine = 0;   // ... that had this tile
-        uint32_t pieces = 0;
         bool ok = true;
         PfPiece p = pf_piece(a.plan, u0, u1);
         if (t == 0 || p.two) load_q(p);
@@ -313,25 +341,31 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                         const unsigned long long mul = at_pair(a.scale2, a.scale2), off = at_pair(-sub, -sub);
                         unsigned long long l2[2] = {0ull, 0ull};
 #pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            uint32_t w[16];
+                        for (int h = 0; h < 8; ++h) {
+                            uint32_t w[8];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int c = 32 * h + 2 * i;
+                            for (int i = 0; i < 8; ++i) {
+                                const int c = 16 * h + 2 * i;
                                 const float2 x = at_unpair(at_fma2(at_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul, off));
-                                w[i] = Act<T>::pack(at_exp2(x.x), at_exp2(x.y));
-                                const float2 f = Act<T>::to_f2(w[i]);
-                                l2[i & 1] = at_add2(l2[i & 1], at_pair(f.x, f.y));
+                                const float y0 = at_exp2(x.x), y1 = at_exp2(x.y);
+                                w[i] = Act<T>::pack(y0, y1);
+                                l2[i & 1] = at_add2(l2[i & 1], at_pair(y0, y1));
                             }
-                            at_st16(ts + 16 * h, w);
+                            pf_st8(ts + 8 * h, w);
+                            if (h == 3) {
+                                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                pf_arrive(pr, lane);
+                            }
                         }
                         const float2 la = at_unpair(at_add2(l2[0], l2[1]));
                         l += la.x + la.y;
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    } else {
+                        pf_arrive(pr, lane);
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(&sh->p_ready[t])) : "memory");
+                    pf_arrive(pr + 8, lane);
                 }
                 if (!ok) break;
             }
@@ -340,8 +374,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
             // the products of this tile's scores have ended (their last commit was waited for): its queries may be replaced
             if (next.unit < u1 && (t == 0 || next.two)) load_q(next);
             if (active) {
-                ok = tc_mbar_wait(tc_smem(&sh->o_done[t]), pieces & 1u, &sh->abort_flag);
-                ++pieces;
+                ok = tc_mbar_wait(tc_smem(&sh->pv_done[t]), (mine - 1) & 1u, &sh->abort_flag);  // (those before it had ended when the last scores were issued)
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const size_t at = (size_t)(blockIdx.x + p.pair) * a.plan.slot_rows + 128 * t + row;
@@ -386,14 +419,21 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
 
 // ------------------------------------------------------------------ own slots, and the sum
 
-constexpr int OW_KEYS = 16, OW_WARPS = 4, OW_THREADS = 32 * OW_WARPS, OW_STAGES = 2;
+constexpr int OW_KEYS = 16, OW_WARPS = 2, OW_THREADS = 32 * OW_WARPS;
 
-template <int DH> constexpr size_t ow_stage_bytes() { return (size_t)2 * OW_KEYS * (DH + 8) * 2; }
-template <int DH> constexpr size_t ow_smem() { return OW_WARPS * OW_STAGES * ow_stage_bytes<DH>(); }  // later the warps' parts: 16 rows of DH f32 each
-template <int DH> constexpr size_t ow_part_bytes() { return (size_t)16 * DH * 4 + 16 * 8; }        // a CTA's part in the first one's memory (clusters)
+// A warp's keys and values: two tiles of keys, one of values.  Small enough for a block beside a block of prefix_tc_kernel, and for eight on an
+// SM of their own.
+template <int DH> constexpr size_t ow_tile_bytes() { return (size_t)OW_KEYS * (DH + 8) * 2; }
+template <int DH> constexpr size_t ow_smem() { return (OW_WARPS * 3 + 1) * ow_tile_bytes<DH>(); }  // and the queries; later the warps' parts: 16 rows of DH f32 each
+template <int DH> constexpr size_t ow_part_bytes() { return (size_t)16 * DH * 4 + 16 * 8; }  // a CTA's part in the first one's memory (clusters)
 
 __device__ __forceinline__ void ow_cp16(void *dst, const void *src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ow_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void ow_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
 }
 __device__ __forceinline__ void ow_ldm4(uint32_t r[4], const void *p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -414,24 +454,87 @@ __device__ __forceinline__ float ow_quad_sum(float v) {
 // factor of a part (m, l, O) in a sum relative to M: a part without a maximum has l = 0 and O = 0, or NaN, which stays
 __device__ __forceinline__ float ow_factor(float m, float M) { return m == -INFINITY ? 1.f : at_exp2(m - M); }
 
-// grid (splits, KV heads, tokens), the splits of a token a cluster
+// a row's part, spread over a warp: PD values per lane
+template <int PD> struct OwPart {
+    float m, l, o[PD];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < PD; ++i) o[i] = 0.f;
+    }
+    __device__ __forceinline__ void add(float pm, float pl, const float *v) {
+        const float M = fmaxf(m, pm), f = ow_factor(m, M), g = ow_factor(pm, M);
+        m = M;
+        l = l * f + pl * g;
+#pragma unroll
+        for (int i = 0; i < PD; ++i) o[i] = o[i] * f + v[i] * g;
+    }
+};
+
+// Adds the prefix's parts of row `row` of a KV head, normalises and stores.  Eight parts at a time, all of whose loads are in flight
+// together: rows are few next to what the memory can hold in flight, and each trip costs a microsecond.
 template <class T, int DH>
-__global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int tokens_per, int splits) {
-    constexpr int ROW = DH + 8, KS = DH / 16, PD = DH / 32;
+__device__ __forceinline__ void ow_finish(const PrefixArgs &a, OwPart<DH / 32> &p, int hkv, int row, int lane) {
+    constexpr int PD = DH / 32, AHEAD = 8;
+    const int group = a.nh / a.nkvh, tok = row / group;
+    if (a.prefix_len) {
+        const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, first = a.plan.first_cta(pair);
+        const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS;
+        const int parts = (int)(a.plan.last_cta(pair) - first) + 1;
+#pragma unroll 1
+        for (int s0 = 0; s0 < parts; s0 += AHEAD) {
+            float v[AHEAD][PD];
+            const float2 x = lane < AHEAD && s0 + lane < parts ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const float *src = a.part_o + (at0 + (size_t)min(s0 + i, parts - 1) * a.plan.slot_rows) * DH;
+                if constexpr (PD == 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(src) + lane);
+                    v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
+                } else {
+                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(src) + lane);
+                    v[i][0] = y.x; v[i][1] = y.y;
+                }
+            }
+            const float M = fmaxf(p.m, warp_max(x.x)), f = ow_factor(p.m, M), g = ow_factor(x.x, M);
+            p.m = M;
+            p.l = p.l * f + warp_sum(x.y * g);
+#pragma unroll
+            for (int d = 0; d < PD; ++d) p.o[d] *= f;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const float w = __shfl_sync(0xffffffffu, g, i);
+                if (s0 + i < parts)
+#pragma unroll
+                    for (int d = 0; d < PD; ++d) p.o[d] = fmaf(v[i][d], w, p.o[d]);
+            }
+        }
+    }
+    const float inv = p.l == 0.f ? 0.f : 1.f / p.l;
+    T *dst = reinterpret_cast<T *>(a.o) + (size_t)tok * a.sto + (size_t)(hkv * group + row % group) * a.sho + lane * PD;
+#pragma unroll
+    for (int i = 0; i < PD; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = Act<T>::pack(p.o[i] * inv, p.o[i + 1] * inv);
+}
+
+// grid (splits, KV heads, tokens); the splits of a token are a cluster where own_kernel adds up
+template <class T, int DH>
+__global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, int tokens_per, int splits) {
+    constexpr int ROW = DH + 8, KS = DH / 16, PD = DH / 32, CH = DH / 8;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float ml[OW_WARPS][16][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, t4 = lane & 3;
     const int hkv = blockIdx.y, t = blockIdx.z, split = blockIdx.x, group = a.nh / a.nkvh;
     const bool first_block = (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
-    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of stores to the first CTA
+    grid_dep_launch();
+    const bool leave = a.prefix_len && a.plan.own_parts, cluster = splits > 1 && !leave;
+    if (cluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of stores to the first CTA
     // consecutive tokens of one sequence, cut at multiples of tokens_per
     const int seq = a.tok_seq[t];
     const bool mine = seq >= 0 && seq < a.n_seq && (t % tokens_per == 0 || a.tok_seq[t - 1] != seq);
     if (!mine) {
-        if (splits > 1) {
-            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        }
-        if (first_block) grid_dep_wait();  // one block at least ends behind the prefix
+        if (cluster) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (first_block) grid_dep_wait();  // the grid ends behind the prefix, whatever its blocks have to do
         return;
     }
     const int most = min(tokens_per - t % tokens_per, a.n - t);
@@ -440,25 +543,20 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
     const uint32_t cap = (uint32_t)a.table_stride << a.page_shift;
     uint32_t ctx = 0;  // of the longest
     if (lane < n_tok) ctx = min(a.tok_ctx[t + lane], cap);
-    const uint32_t r0 = (uint32_t)gid, r1 = r0 + 8;  // this thread's rows
-    const uint32_t lim0 = __shfl_sync(0xffffffffu, ctx, (int)(r0 / group) & 31), lim1 = __shfl_sync(0xffffffffu, ctx, (int)(r1 / group) & 31);
+    const int r0 = gid, r1 = gid + 8;  // this thread's rows
+    const uint32_t lim0 = __shfl_sync(0xffffffffu, ctx, r0 / group), lim1 = __shfl_sync(0xffffffffu, ctx, r1 / group);  // 0 behind the last row
     const uint32_t lim_min = __reduce_min_sync(0xffffffffu, lane < n_tok ? ctx : 0xffffffffu);
     ctx = __reduce_max_sync(0xffffffffu, ctx);
     const int chunks = (int)((ctx + OW_KEYS - 1) / OW_KEYS);
 
-    uint32_t qa[KS][4];
-    {
-        auto row_of = [&](int r) { return reinterpret_cast<const T *>(a.q) + (size_t)(t + r / group) * a.stq + (size_t)(hkv * group + r % group) * a.shq; };
-        const T *q0 = row_of((int)r0 < rows ? (int)r0 : 0), *q1 = row_of((int)r1 < rows ? (int)r1 : 0);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qa[k][0] = *reinterpret_cast<const uint32_t *>(q0 + 16 * k + 2 * t4);
-            qa[k][1] = *reinterpret_cast<const uint32_t *>(q1 + 16 * k + 2 * t4);
-            qa[k][2] = *reinterpret_cast<const uint32_t *>(q0 + 16 * k + 8 + 2 * t4);
-            qa[k][3] = *reinterpret_cast<const uint32_t *>(q1 + 16 * k + 8 + 2 * t4);
-        }
+    T *const qs = reinterpret_cast<T *>(smem + OW_WARPS * 3 * ow_tile_bytes<DH>());  // [16][ROW], rows behind the last are zero
+    for (int i = tid; i < 16 * CH; i += OW_THREADS) {
+        const int r = i / CH, c = 8 * (i % CH);
+        const bool valid = r < rows;
+        ow_cp16(qs + r * ROW + c, reinterpret_cast<const T *>(a.q) + (valid ? (size_t)(t + r / group) * a.stq + (size_t)(hkv * group + r % group) * a.shq + c : 0), valid);
     }
-    unsigned char *ring = smem + (size_t)warp * OW_STAGES * ow_stage_bytes<DH>();
+    ow_commit();
+    T *const k_tiles = reinterpret_cast<T *>(smem + (size_t)warp * 3 * ow_tile_bytes<DH>()), *const vs = k_tiles + 2 * OW_KEYS * ROW;
     const int step = splits * OW_WARPS;
     auto row_at = [&](int chunk) -> long long {  // lane i: where key i of the chunk lies, -1: nowhere
         const uint32_t key = (uint32_t)chunk * OW_KEYS + (lane & 15);
@@ -467,46 +565,45 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
         if (page < 0 || page >= a.pages.n_pages) return -1;
         return (long long)page * a.pages.stride_page + (long long)(key & ((1u << a.page_shift) - 1)) * a.pages.stride_tok + (long long)hkv * a.pages.stride_head;
     };
-    auto request = [&](int stage, long long at) {
-        T *ks = reinterpret_cast<T *>(ring + (size_t)stage * ow_stage_bytes<DH>()), *vs = ks + OW_KEYS * ROW;
-        constexpr int CH = DH / 8;
+    auto request = [&](T *dst, const void *base, long long at) {
 #pragma unroll
         for (int i = 0; i < OW_KEYS * CH / 32; ++i) {
             const int key = lane / CH + i * (32 / CH), c = 8 * (lane % CH);
             const long long off = __shfl_sync(0xffffffffu, at, key);
-            ow_cp16(ks + key * ROW + c, reinterpret_cast<const T *>(a.pages.k) + (off < 0 ? 0 : off + c), off >= 0);
-            ow_cp16(vs + key * ROW + c, reinterpret_cast<const T *>(a.pages.v) + (off < 0 ? 0 : off + c), off >= 0);
+            ow_cp16(dst + key * ROW + c, reinterpret_cast<const T *>(base) + (off < 0 ? 0 : off + c), off >= 0);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     float o[DH / 8][4];
 #pragma unroll
     for (int i = 0; i < DH / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    // Copies in flight, in this order: keys of this chunk, its values, keys of the next; page ids of the one behind.
     const int c0 = split * OW_WARPS + warp;
-    long long at = row_at(c0), ahead = row_at(c0 + step);
-    unsigned there = __ballot_sync(0xffffffffu, at >= 0);
-    if (c0 < chunks) request(0, at);
-    int stage = 0;
+    long long at0 = row_at(c0), at1 = row_at(c0 + step), at2 = row_at(c0 + 2 * step);
+    if (c0 < chunks) {
+        request(k_tiles, a.pages.k, at0);
+        ow_commit();
+        request(vs, a.pages.v, at0);
+        ow_commit();
+        request(k_tiles + OW_KEYS * ROW, a.pages.k, at1);
+        ow_commit();
+    }
+    if (c0 < chunks) ow_wait<3>();
+    else ow_wait<0>();
+    __syncthreads();  // the queries are there
+    int tile = 0;
     for (int c = c0; c < chunks; c += step) {
-        at = ahead;
-        ahead = row_at(c + 2 * step);
-        const unsigned there_next = __ballot_sync(0xffffffffu, at >= 0);
-        if (c + step < chunks) {
-            request(stage ^ 1, at);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        __syncwarp();
-        const T *ks = reinterpret_cast<const T *>(ring + (size_t)stage * ow_stage_bytes<DH>()), *vs = ks + OW_KEYS * ROW;
+        const unsigned there = __ballot_sync(0xffffffffu, at0 >= 0);
+        const T *ks = k_tiles + tile * OW_KEYS * ROW;
+        ow_wait<2>();
         float s[2][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            uint32_t b[4];
+            uint32_t qa[4], b[4];
+            ow_ldm4(qa, qs + (lane & 15) * ROW + 16 * k + (lane >> 4) * 8);
             ow_ldm4(b, ks + ((lane & 7) + (lane >> 4) * 8) * ROW + 16 * k + (lane >> 3 & 1) * 8);
-            mma16816<T>(s[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[0], b[1]);
-            mma16816<T>(s[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[2], b[3]);
+            mma16816<T>(s[0], qa[0], qa[1], qa[2], qa[3], b[0], b[1]);
+            mma16816<T>(s[1], qa[0], qa[1], qa[2], qa[3], b[2], b[3]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -525,13 +622,14 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
         m0 = n0;
         m1 = n1;
         uint32_t pa[4];
-        pa[0] = Act<T>::pack(at_exp2(s[0][0] - b0), at_exp2(s[0][1] - b0));
-        pa[1] = Act<T>::pack(at_exp2(s[0][2] - b1), at_exp2(s[0][3] - b1));
-        pa[2] = Act<T>::pack(at_exp2(s[1][0] - b0), at_exp2(s[1][1] - b0));
-        pa[3] = Act<T>::pack(at_exp2(s[1][2] - b1), at_exp2(s[1][3] - b1));
-        const float2 w0 = Act<T>::to_f2(pa[0]), w1 = Act<T>::to_f2(pa[1]), w2 = Act<T>::to_f2(pa[2]), w3 = Act<T>::to_f2(pa[3]);
-        l0 = l0 * f0 + ((w0.x + w0.y) + (w2.x + w2.y));
-        l1 = l1 * f1 + ((w1.x + w1.y) + (w3.x + w3.y));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float x0 = at_exp2(s[h][0] - b0), x1 = at_exp2(s[h][1] - b0), y0 = at_exp2(s[h][2] - b1), y1 = at_exp2(s[h][3] - b1);
+            l0 = (h ? l0 : l0 * f0) + (x0 + x1);
+            l1 = (h ? l1 : l1 * f1) + (y0 + y1);
+            pa[2 * h] = Act<T>::pack(x0, x1);
+            pa[2 * h + 1] = Act<T>::pack(y0, y1);
+        }
         if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
 #pragma unroll
             for (int i = 0; i < DH / 8; ++i) {
@@ -541,6 +639,7 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
                 o[i][3] *= f1;
             }
         }
+        ow_wait<1>();
         // Keys that one token of the group sees and another does not: a weight of zero times a value that is not finite would be NaN.
         bool odd = false;
         if ((uint32_t)(c + 1) * OW_KEYS > lim_min && lim_min < ctx)
@@ -577,13 +676,20 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
             mma16816<T>(o[2 * i], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
             mma16816<T>(o[2 * i + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
         }
-        __syncwarp();  // the stage may be filled again
-        there = there_next;
-        stage ^= 1;
+        __syncwarp();  // values and this tile of keys may be replaced
+        request(vs, a.pages.v, at1);
+        ow_commit();
+        request(k_tiles + tile * OW_KEYS * ROW, a.pages.k, at2);
+        ow_commit();
+        at0 = at1;
+        at1 = at2;
+        at2 = row_at(c + 3 * step);
+        tile ^= 1;
     }
+    ow_wait<0>();
     l0 = ow_quad_sum(l0);
     l1 = ow_quad_sum(l1);
-    __syncthreads();  // the rings are done with: the warps' parts go there
+    __syncthreads();  // the tiles are done with: the warps' parts go there
     float *parts = reinterpret_cast<float *>(smem);  // [warp][16][DH]
     if (t4 == 0) {
         ml[warp][gid][0] = m0;
@@ -598,110 +704,85 @@ __global__ void __launch_bounds__(OW_THREADS) own_kernel(const PrefixArgs a, int
         *reinterpret_cast<float2 *>(d + 8 * DH) = make_float2(o[i][2], o[i][3]);
     }
     __syncthreads();
-    // a warp per row from here on, PD values per lane
-    struct Part {
-        float m, l, o[PD];
+    // a warp per row from here on
+    auto both = [&](int r) {  // the two warps' parts of a row
+        OwPart<PD> p;
+        p.clear();
+#pragma unroll
+        for (int w = 0; w < OW_WARPS; ++w) p.add(ml[w][r][0], ml[w][r][1], parts + ((size_t)w * 16 + r) * DH + lane * PD);
+        return p;
     };
-    auto add = [&](Part &p, float m, float l, const float *v) {  // v: this lane's PD values
-        const float M = fmaxf(p.m, m), f = ow_factor(p.m, M), g = ow_factor(m, M);
-        p.m = M;
-        p.l = p.l * f + l * g;
-#pragma unroll
-        for (int i = 0; i < PD; ++i) p.o[i] = p.o[i] * f + v[i] * g;
-    };
-    float *cluster_o = reinterpret_cast<float *>(smem + ow_smem<DH>());  // first split: [split][16][DH], then (m, l) [split][16]
-    float *cluster_ml = cluster_o + (size_t)splits * 16 * DH;
-    if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    Part held[16 / OW_WARPS];
-#pragma unroll
-    for (int k = 0; k < 16 / OW_WARPS; ++k) {
-        const int r = warp + OW_WARPS * k;
-        Part &p = held[k];
-        p.m = -INFINITY;
-        p.l = 0.f;
-#pragma unroll
-        for (int i = 0; i < PD; ++i) p.o[i] = 0.f;
-        if (r >= rows) continue;
-#pragma unroll
-        for (int w = 0; w < OW_WARPS; ++w) add(p, ml[w][r][0], ml[w][r][1], parts + ((size_t)w * 16 + r) * DH + lane * PD);
-        if (splits > 1) {
+    if (cluster) {
+        float *const cluster_o = reinterpret_cast<float *>(smem + ow_smem<DH>());  // in the first CTA: [split][16][DH], then (m, l) [split][16]
+        float *const cluster_ml = cluster_o + (size_t)splits * 16 * DH;
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+#pragma unroll 1
+        for (int r = warp; r < rows; r += OW_WARPS) {
+            const OwPart<PD> p = both(r);
             uint32_t peer;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"((uint32_t)__cvta_generic_to_shared(cluster_o + ((size_t)split * 16 + r) * DH + lane * PD)), "r"(0));
 #pragma unroll
             for (int i = 0; i < PD; ++i) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer + 4 * i), "f"(p.o[i]) : "memory");
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"((uint32_t)__cvta_generic_to_shared(cluster_ml + ((size_t)split * 16 + r) * 2)), "r"(0));
             if (lane == 0) asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer), "f"(p.m), "f"(p.l) : "memory");
+            __syncwarp();
         }
-    }
-    if (splits > 1) {
-        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (split != 0) return;
-#pragma unroll
-        for (int k = 0; k < 16 / OW_WARPS; ++k) {
-            const int r = warp + OW_WARPS * k;
-            if (r >= rows) continue;
-            for (int s = 1; s < splits; ++s) add(held[k], cluster_ml[(s * 16 + r) * 2], cluster_ml[(s * 16 + r) * 2 + 1], cluster_o + ((size_t)s * 16 + r) * DH + lane * PD);
+        grid_dep_wait();
+#pragma unroll 1
+        for (int r = warp; r < rows; r += OW_WARPS) {
+            OwPart<PD> p;
+            p.clear();
+            for (int s = 0; s < splits; ++s) p.add(cluster_ml[(s * 16 + r) * 2], cluster_ml[(s * 16 + r) * 2 + 1], cluster_o + ((size_t)s * 16 + r) * DH + lane * PD);
+            ow_finish<T, DH>(a, p, hkv, t * group + r, lane);
         }
+        return;
+    }
+    if (leave) {  // own_sum_kernel adds up
+#pragma unroll 1
+        for (int r = warp; r < rows; r += OW_WARPS) {
+            const OwPart<PD> p = both(r);
+            const size_t at = a.own_row + ((size_t)split * a.nkvh + hkv) * a.plan.rows + t * group + r;
+            if (lane == 0) a.part_ml[at] = make_float2(p.m, p.l);
+#pragma unroll
+            for (int i = 0; i < PD; i += 2) *reinterpret_cast<float2 *>(a.part_o + at * DH + lane * PD + i) = make_float2(p.o[i], p.o[i + 1]);
+        }
+        if (first_block) grid_dep_wait();
+        return;
     }
     grid_dep_wait();  // the parts of the prefix
-#pragma unroll
-    for (int k = 0; k < 16 / OW_WARPS; ++k) {
-        const int r = warp + OW_WARPS * k;
-        if (r >= rows) continue;
-        Part &p = held[k];
-        const int tok = t + r / group, g = r % group;
-        if (a.prefix_len) {
-            const int row = tok * group + g;  // of the KV head
-            const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, last = a.plan.last_cta(pair);
-            // all maxima first, a part per lane, then the parts four at a time: two round trips for up to 32 parts
-            const long long first = a.plan.first_cta(pair);
-            const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS;
-            const int parts_n = (int)(last - first) + 1;
-            float M = p.m;
-            float2 x = make_float2(-INFINITY, 0.f);
-            for (int s0 = 0; s0 < parts_n; s0 += 32) {
-                x = s0 + lane < parts_n ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
-                M = fmaxf(M, warp_max(x.x));
-            }
-            const float f = ow_factor(p.m, M);
-            p.l *= f;
-#pragma unroll
-            for (int i = 0; i < PD; ++i) p.o[i] *= f;
-            for (int s0 = 0; s0 < parts_n; s0 += 32) {
-                if (parts_n > 32) x = s0 + lane < parts_n ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
-                const float g = ow_factor(x.x, M);
-                p.l += warp_sum(x.y * g);
-                const int m = min(32, parts_n - s0);
 #pragma unroll 1
-                for (int s = 0; s < m; s += 4) {
-                    float v[4][PD];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float *src = a.part_o + (at0 + (size_t)(s0 + min(s + i, m - 1)) * a.plan.slot_rows) * DH;
-                        if constexpr (PD == 4) {
-                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(src) + lane);
-                            v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
-                        } else {
-                            const float2 y = __ldcg(reinterpret_cast<const float2 *>(src) + lane);
-                            v[i][0] = y.x; v[i][1] = y.y;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float w = __shfl_sync(0xffffffffu, g, s + i & 31);
-                        if (s + i < m)
-#pragma unroll
-                            for (int d = 0; d < PD; ++d) p.o[d] = fmaf(v[i][d], w, p.o[d]);
-                    }
-                }
-            }
-        }
-        const float inv = p.l == 0.f ? 0.f : 1.f / p.l;
-        T *dst = reinterpret_cast<T *>(a.o) + (size_t)tok * a.sto + (size_t)(hkv * group + g) * a.sho + lane * PD;
-#pragma unroll
-        for (int i = 0; i < PD; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = Act<T>::pack(p.o[i] * inv, p.o[i + 1] * inv);
+    for (int r = warp; r < rows; r += OW_WARPS) {
+        OwPart<PD> p = both(r);
+        ow_finish<T, DH>(a, p, hkv, t * group + r, lane);
     }
+}
+
+// Sum of a row's own part and the prefix's: a warp per row, behind own_kernel (which ends behind the prefix).
+template <class T, int DH>
+__global__ void __launch_bounds__(256) own_sum_kernel(const PrefixArgs a, int splits) {
+    constexpr int PD = DH / 32;
+    const int lane = threadIdx.x & 31, hkv = blockIdx.y, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= a.plan.rows) return;
+    const int seq = a.tok_seq[row / (a.nh / a.nkvh)];
+    if (seq < 0 || seq >= a.n_seq) return;
+    grid_dep_wait();
+    OwPart<PD> p;
+    p.clear();
+    for (int i = 0; i < splits; ++i) {
+        const size_t at = a.own_row + ((size_t)i * a.nkvh + hkv) * a.plan.rows + row;
+        const float2 x = __ldcg(a.part_ml + at);
+        float v[PD];
+#pragma unroll
+        for (int d = 0; d < PD; d += 2) {
+            const float2 y = __ldcg(reinterpret_cast<const float2 *>(a.part_o + at * DH + lane * PD + d));
+            v[d] = y.x;
+            v[d + 1] = y.y;
+        }
+        p.add(x.x, x.y, v);
+    }
+    ow_finish<T, DH>(a, p, hkv, row, lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -729,12 +810,16 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
         LCU_CHECK_CUDA(launch_kernel(prefix_tc_kernel<T, DH>, dim3(a.plan.ctas), dim3(PF_THREADS), pf_smem<DH>(), s, false, a, mk, mv, dt == LCU_BF16 ? 1u : 0u));
     }
     const int group = a.nh / a.nkvh, tokens_per = 16 / group;
-    // long contexts of few tokens: their keys over a cluster
+    // keys of long contexts: over a cluster where blocks are few, over blocks that leave a part each where there are more
     const long long cap = (long long)a.table_stride << a.page_shift, blocks = (long long)a.nkvh * a.n;
+    const bool leave = a.prefix_len && a.plan.own_parts;
     int splits = 1;
-    while (splits < 8 && blocks * splits * 2 <= 2LL * sm_count() && cap > (long long)splits * 128) splits *= 2;
-    const size_t smem = ow_smem<DH>() + (splits > 1 ? splits * ow_part_bytes<DH>() : 0);
+    if (leave) splits = (int)(cap < 64LL * a.plan.own_parts ? (cap + 63) / 64 > 0 ? (cap + 63) / 64 : 1 : a.plan.own_parts);
+    else while (splits < 8 && blocks * splits <= sm_count() && cap > (long long)splits * 64) splits *= 2;
+    const size_t smem = ow_smem<DH>() + (splits > 1 && !leave ? splits * ow_part_bytes<DH>() : 0);
     LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>() + 8 * ow_part_bytes<DH>())));
+    LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.nkvh, a.n);
     cfg.blockDim = dim3(OW_THREADS);
@@ -742,7 +827,7 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
-    if (splits > 1) {
+    if (splits > 1 && !leave) {
         attr[n_attr].id = cudaLaunchAttributeClusterDimension;
         attr[n_attr].val.clusterDim.x = splits;
         attr[n_attr].val.clusterDim.y = attr[n_attr].val.clusterDim.z = 1;
@@ -756,6 +841,7 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
     LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, own_kernel<T, DH>, (const PrefixArgs)a, tokens_per, splits));
+    if (leave) LCU_CHECK_CUDA(launch_kernel(own_sum_kernel<T, DH>, dim3((a.plan.rows + 7) / 8, a.nkvh), dim3(256), 0, s, true, a, splits));
     return LCU_OK;
 }
 
@@ -765,7 +851,7 @@ using namespace lcu;
 
 extern "C" size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len) {
     if (n <= 0 || nkvh <= 0 || nh < nkvh || nh % nkvh || dh <= 0 || !prefix_len) return 0;
-    return prefix_bytes(prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count()), dh);
+    return prefix_bytes(prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count()), nkvh, dh);
 }
 
 extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q, int stq, int shq, const lcu_kv_pages *pages, const int32_t *prefix_table,
@@ -798,7 +884,8 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     if (prefix_len) {
         a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count());
         a.part_ml = reinterpret_cast<float2 *>(workspace);
-        a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan));
+        a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan, nkvh));
+        a.own_row = prefix_own_row(a.plan);
     }
     if (dt == LCU_F16) return dh == 64 ? prefix_run<__half, 64>(a, dt, as_stream(s)) : prefix_run<__half, 128>(a, dt, as_stream(s));
     return dh == 64 ? prefix_run<__nv_bfloat16, 64>(a, dt, as_stream(s)) : prefix_run<__nv_bfloat16, 128>(a, dt, as_stream(s));

@@ -22,6 +22,9 @@ struct PrefixPlan {
     long long pairs, units, per;  // (KV head, row tile); all units; units of a CTA
     int ctas;
     int slot_rows;   // rows of a piece's slot
+    // More (KV head, token) blocks for the own slots than SMs: they leave their parts too, at most so many of a row, and a kernel of its
+    // own adds up.  (A block that adds up waits for the prefix, and would hold its place beside it from the blocks that have not begun.)
+    int own_parts;
 
     LCU_HD long long first_cta(long long pair) const { return pair * key_tiles / per; }
     LCU_HD long long last_cta(long long pair) const { return ((pair + 1) * key_tiles - 1) / per; }
@@ -39,11 +42,15 @@ inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, i
     p.per = (p.units + sms - 1) / sms;
     p.ctas = (int)((p.units + p.per - 1) / p.per);
     p.slot_rows = p.rows < PF_ROWS ? p.rows : PF_ROWS;
+    const long long blocks = (long long)n * nkvh;
+    p.own_parts = blocks <= sms ? 0 : blocks >= 6LL * sms ? 1 : (int)(6LL * sms / blocks);
     return p;
 }
 
-// Workspace: (maximum, sum) of every row of every slot, then the rows' unnormalised outputs.
-inline size_t prefix_ml_bytes(const PrefixPlan &p) { return ((size_t)p.slots() * p.slot_rows * 8 + 255) / 256 * 256; }
-inline size_t prefix_bytes(const PrefixPlan &p, int dh) { return prefix_ml_bytes(p) + (size_t)p.slots() * p.slot_rows * dh * 4; }
+// Workspace, in rows: those of every slot, then those of the own parts, [part][KV head][row].  (maximum, sum) of each, then their unnormalised outputs.
+inline size_t prefix_own_row(const PrefixPlan &p) { return (size_t)p.slots() * p.slot_rows; }
+inline size_t prefix_part_rows(const PrefixPlan &p, int nkvh) { return prefix_own_row(p) + (size_t)p.own_parts * nkvh * p.rows; }
+inline size_t prefix_ml_bytes(const PrefixPlan &p, int nkvh) { return (prefix_part_rows(p, nkvh) * 8 + 255) / 256 * 256; }
+inline size_t prefix_bytes(const PrefixPlan &p, int nkvh, int dh) { return prefix_ml_bytes(p, nkvh) + prefix_part_rows(p, nkvh) * dh * 4; }
 
 }  // namespace lcu

@@ -1,6 +1,6 @@
 // From logits to the tokens that a verified draft leaves (no counterpart in the reference, which samples one token per row,
 // exec/output_head.rs:104-113): probabilities of rows of logits, and the acceptance of drafted tokens against them.
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace lcu {
 
@@ -19,6 +19,10 @@ __device__ __forceinline__ uint32_t vf_peer(const void *local, uint32_t cta) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(la), "r"(cta));
     return ra;
 }
+// ... and counts 8 bytes on the peer's barrier: no fence, so nobody waits for stores to global memory that are still on their way
+__device__ __forceinline__ void vf_st_async(uint32_t ra, unsigned long long v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u64 [%0], %1, [%2];" ::"r"(ra), "l"(v), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void vf_st_peer(uint32_t ra, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ra), "l"(v) : "memory"); }
 
 template <class T> __device__ __forceinline__ float vf_f(T v) { return Act<T>::to_f(v); }
@@ -30,7 +34,9 @@ template <> __device__ __forceinline__ float vf_f<float>(float v) { return v; }
 //
 // Bound by HBM: a row is read once and written once.  A thread-block cluster of up to 8 CTAs takes a row and keeps its values in
 // registers between the two halves (vocabularies up to 131072; longer rows are read a second time, from L2); maxima and sums, relative
-// to each CTA's own maximum, cross the cluster as pairs in one exchange.
+// to each CTA's own maximum, cross the cluster as pairs in one exchange.  Where there are more rows than clusters at once, clusters stay and each
+// CTA requests its part of the next row (one bulk copy into shared memory) as soon as it has taken up this one: the memory works on
+// while maxima, exponentials and sums wait for one another.
 struct SoftmaxArgs {
     float *probs;
     size_t stride_p;
@@ -38,9 +44,15 @@ struct SoftmaxArgs {
     size_t stride_l;
     const float *temperature;
     size_t n, slice;  // values of a row, of a CTA
+    int rows;
 };
 
-__device__ __forceinline__ float sm_exp(float x, float m, float inv_t) { return expf((x - m) * inv_t); }
+// 2^((x - m) c), c = log2(e) / T: the difference first, so that what is rounded shrinks with it; off by 2^-22 and 3 |z| 2^-24 relatively
+__device__ __forceinline__ float sm_exp(float x, float m, float c) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"((x - m) * c));
+    return r;
+}
 
 // (value, index) as one number that grows with the value and, among equals, with a lower index; NaN is below everything
 __device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
@@ -50,50 +62,35 @@ __device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
     return ((unsigned long long)u << 32) | (uint32_t)~i;
 }
 
-template <class T, bool VEC, int EPT>
-__global__ void __launch_bounds__(SM_THREADS) softmax_kernel(const SoftmaxArgs a) {
+// grid (CTAs of a cluster, clusters)
+template <class T, bool VEC, int EPT, bool AHEAD>
+__global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArgs a) {
     constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    __shared__ unsigned long long part[SM_THREADS / 32], xchg[VF_CLUSTER];
+    extern __shared__ __align__(16) unsigned char staged[];  // AHEAD: this CTA's part of the next row
+    __shared__ unsigned long long part[SM_THREADS / 32], xchg[2][VF_CLUSTER], xbar[2], bar;
+    __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = vf_rank(), size = gridDim.x;
-    const int row = blockIdx.y;
-    vf_cluster_arrive();  // waited for ahead of the exchange: a peer's shared memory is there once it runs
-    const T *x = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.stride_l;
-    float *out = a.probs + (size_t)row * a.stride_p;
+    if (tid == 0) {
+        abort_flag = 0;
+        tc_mbar_init(tc_smem(&bar), 1);
+        tc_mbar_init(tc_smem(&xbar[0]), 1);
+        tc_mbar_init(tc_smem(&xbar[1]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    vf_cluster_arrive();  // waited for ahead of the first exchange: a peer's shared memory is there once it runs, its barriers once it arrives
     const size_t lo = (size_t)rank * a.slice < a.n ? (size_t)rank * a.slice : a.n, hi = lo + a.slice < a.n ? lo + a.slice : a.n;
-    const float t = a.temperature ? a.temperature[row] : 1.f;
-    const float inv_t = 1.f / t > 3.0e38f ? 3.0e38f : 1.f / t;  // (x - m) / T stays 0 where x = m, however small T
-
-    auto load = [&](size_t i, float *f) {  // V values from i on; -inf behind the row
-        if (VEC && i + V <= hi) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(x + i);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) f[k] = __uint_as_float(w[k]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; k += 2) {
-                    const float2 p = Act<T>::to_f2(w[k / 2]);
-                    f[k] = p.x;
-                    f[k + 1] = p.y;
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = i + k < hi ? vf_f<T>(x[i + k]) : -INFINITY;
+    const size_t whole = AHEAD ? lo + (hi - lo) / V * V : lo;  // values below it come through shared memory
+    const T *base = reinterpret_cast<const T *>(a.logits);
+    auto request = [&](int row) {
+        const uint32_t bytes = (uint32_t)((whole - lo) * sizeof(T));
+        if (!AHEAD || tid != 0 || bytes == 0 || row >= a.rows) return;
+        tc_mbar_expect_tx(tc_smem(&bar), bytes);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(tc_smem(staged)), "l"(base + (size_t)row * a.stride_l + lo), "r"(bytes), "r"(tc_smem(&bar)) : "memory");
     };
-    auto store = [&](size_t i, const float *f) {
-        if (VEC && i + V <= hi) {
-#pragma unroll
-            for (int k = 0; k < V; k += 4) __stcs(reinterpret_cast<float4 *>(out + i + k), make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]));
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (i + k < hi) __stcs(out + i + k, f[k]);
-    };
+    request(blockIdx.y);
     auto combine = [&](unsigned long long v, auto op) {  // over the block
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -105,96 +102,149 @@ __global__ void __launch_bounds__(SM_THREADS) softmax_kernel(const SoftmaxArgs a
         __syncthreads();
         return v;
     };
-    auto exchange = [&](unsigned long long v) {  // into everyone's xchg
-        vf_cluster_wait();
-        if (tid < (int)size) vf_st_peer(vf_peer(&xchg[rank], (uint32_t)tid), v);
-        __syncwarp();
-        vf_cluster_arrive();
-        vf_cluster_wait();
+    // Into everyone's slots, in turns.  A peer writes a turn's slots again only two rows on, and by then it has had this CTA's value of the row
+    // between, which is sent behind the last read of these.
+    uint32_t turn = 0, phase = 0;
+    bool begun = false;
+    auto exchange = [&](unsigned long long v) {
+        if (!begun) vf_cluster_wait();
+        begun = true;
+        if (tid == 0) tc_mbar_expect_tx(tc_smem(&xbar[turn]), 8 * size);
+        if (tid < (int)size) vf_st_async(vf_peer(&xchg[turn][rank], (uint32_t)tid), v, vf_peer(&xbar[turn], (uint32_t)tid));
+        const bool ok = tc_mbar_wait(tc_smem(&xbar[turn]), phase, &abort_flag);
+        if (!ok) abort_flag = 1;
+        return ok;
     };
     auto greater = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
+    const size_t first = lo + (size_t)tid * V;
+    constexpr size_t step = (size_t)SM_THREADS * V;
 
-    float keep[EPT > 0 ? EPT : V];
-    const size_t first = lo + (size_t)tid * V, step = (size_t)SM_THREADS * V;
-    if (t == 0.f) {  // (uniform over the cluster)
-        unsigned long long best = 0;
-        for (size_t i = first; i < hi; i += step) {
-            load(i, keep);
+    for (int row = blockIdx.y; row < a.rows; row += gridDim.y, phase ^= turn, turn ^= 1u) {
+        const T *x = base + (size_t)row * a.stride_l;
+        float *out = a.probs + (size_t)row * a.stride_p;
+        const float t = a.temperature ? a.temperature[row] : 1.f;
+        const float inv_t = 1.f / t > 2.0e38f ? 2.0e38f * 1.442695041f : 1.442695041f / t;  // finite: (x - m) / T stays 0 where x = m, however small T
+        bool here = true;
+        if constexpr (AHEAD) here = whole == lo || tc_mbar_wait(tc_smem(&bar), turn, &abort_flag);
+        if (!here) abort_flag = 1;
+        auto load = [&](size_t i, float *f) {  // V values from i on; -inf behind the slice
+            if (VEC && i + V <= hi) {
+                const uint4 q = AHEAD ? *reinterpret_cast<const uint4 *>(staged + (i - lo) * sizeof(T)) : *reinterpret_cast<const uint4 *>(x + i);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) f[k] = __uint_as_float(w[k]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; k += 2) {
+                        const float2 p = Act<T>::to_f2(w[k / 2]);
+                        f[k] = p.x;
+                        f[k + 1] = p.y;
+                    }
+                }
+                return;
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = i + k < hi ? vf_f<T>(x[i + k]) : -INFINITY;
+        };
+        auto store = [&](size_t i, const float *f) {
+            if (VEC && i + V <= hi) {
+#pragma unroll
+                for (int k = 0; k < V; k += 4) __stcs(reinterpret_cast<float4 *>(out + i + k), make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]));
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (i + k < hi) best = greater(best, sm_key(keep[k], (uint32_t)(i + k)));
-        }
-        exchange(combine(best, greater));
-        best = 0;
-        for (uint32_t c = 0; c < size; ++c) best = greater(best, xchg[c]);
-        // a row of -inf (and NaN) alone has no largest
-        const bool some = (uint32_t)(best >> 32) > 0x007fffffu;
-        const size_t at = some ? (size_t)(uint32_t)~(uint32_t)best : a.n;
-        for (size_t i = first; i < hi; i += step) {
+                if (i + k < hi) __stcs(out + i + k, f[k]);
+        };
+        float keep[EPT > 0 ? EPT : V];
+        if (t == 0.f) {  // (uniform over the cluster)
+            unsigned long long best = 0;
+            for (size_t i = first; i < hi; i += step) {
+                load(i, keep);
 #pragma unroll
-            for (int k = 0; k < V; ++k) keep[k] = i + k == at ? 1.f : 0.f;
-            store(i, keep);
+                for (int k = 0; k < V; ++k)
+                    if (i + k < hi) best = greater(best, sm_key(keep[k], (uint32_t)(i + k)));
+            }
+            best = combine(best, greater);
+            request(row + gridDim.y);
+            here = exchange(best) && here;
+            best = 0;
+            for (uint32_t c = 0; c < size; ++c) best = greater(best, xchg[turn][c]);
+            // a row of -inf (and NaN) alone has no largest
+            const bool some = (uint32_t)(best >> 32) > 0x007fffffu;
+            const size_t at = some ? (size_t)(uint32_t)~(uint32_t)best : a.n;
+            for (size_t i = first; i < hi; i += step) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) keep[k] = !here ? __int_as_float(0x7fc00000) : i + k == at ? 1.f : 0.f;
+                store(i, keep);
+            }
+            continue;
         }
-        return;
+        float m = -INFINITY;
+        if constexpr (EPT > 0) {
+#pragma unroll
+            for (int j = 0; j < EPT / V; ++j) load(first + j * step, keep + j * V);
+            if (AHEAD && !here) keep[0] = __int_as_float(0x7fc00000);  // the copy never came: the row becomes NaN
+#pragma unroll
+            for (int j = 0; j < EPT; ++j) m = fmaxf(m, keep[j]);
+        } else {
+            for (size_t i = first; i < hi; i += step) {
+                load(i, keep);
+#pragma unroll
+                for (int k = 0; k < V; ++k) m = fmaxf(m, keep[k]);
+            }
+        }
+        m = __uint_as_float((uint32_t)combine(__float_as_uint(m), [](unsigned long long p, unsigned long long q) {
+            return (unsigned long long)__float_as_uint(fmaxf(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)q)));
+        }));
+        request(row + gridDim.y);  // everyone has taken this row up
+        const float off = m == -INFINITY ? 0.f : m;
+        float s = 0.f;
+        if constexpr (EPT > 0) {
+#pragma unroll
+            for (int j = 0; j < EPT; ++j) {
+                keep[j] = sm_exp(keep[j], off, inv_t);
+                s += keep[j];
+            }
+        } else {
+            for (size_t i = first; i < hi; i += step) {
+                load(i, keep);
+#pragma unroll
+                for (int k = 0; k < V; ++k) s += sm_exp(keep[k], off, inv_t);
+            }
+        }
+        s = __uint_as_float((uint32_t)combine(__float_as_uint(s), [](unsigned long long p, unsigned long long q) {
+            return (unsigned long long)__float_as_uint(__uint_as_float((uint32_t)p) + __uint_as_float((uint32_t)q));
+        }));
+        if (!exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s))) s = __int_as_float(0x7fc00000);
+        float top = -INFINITY, sum = 0.f;
+        for (uint32_t c = 0; c < size; ++c) top = fmaxf(top, __uint_as_float((uint32_t)(xchg[turn][c] >> 32)));
+        for (uint32_t c = 0; c < size; ++c) {
+            const float mc = __uint_as_float((uint32_t)(xchg[turn][c] >> 32)), sc = __uint_as_float((uint32_t)xchg[turn][c]);
+            sum += mc == -INFINITY ? sc : sc * sm_exp(mc, top, inv_t);  // (a slice of -inf has sum 0, or NaN where it holds one)
+        }
+        const float inv = sum == 0.f ? 0.f : s != s ? s : 1.f / sum;  // (NaN among this CTA's values, or a peer that never came)
+        if constexpr (EPT > 0) {
+            const float f = (m == -INFINITY ? 1.f : sm_exp(m, top, inv_t)) * inv;
+#pragma unroll
+            for (int j = 0; j < EPT; ++j) keep[j] *= f;
+#pragma unroll
+            for (int j = 0; j < EPT / V; ++j)
+                if (first + j * step < hi) store(first + j * step, keep + j * V);
+        } else {
+            const float b = top == -INFINITY ? 0.f : top;
+            for (size_t i = first; i < hi; i += step) {
+                load(i, keep);
+#pragma unroll
+                for (int k = 0; k < V; ++k) keep[k] = sm_exp(keep[k], b, inv_t) * inv;
+                store(i, keep);
+            }
+        }
     }
-    float m = -INFINITY;
-    if constexpr (EPT > 0) {
-#pragma unroll
-        for (int j = 0; j < EPT / V; ++j) load(first + j * step, keep + j * V);
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) m = fmaxf(m, keep[j]);
-    } else {
-        for (size_t i = first; i < hi; i += step) {
-            load(i, keep);
-#pragma unroll
-            for (int k = 0; k < V; ++k) m = fmaxf(m, keep[k]);
-        }
-    }
-    m = __uint_as_float((uint32_t)combine(__float_as_uint(m), [](unsigned long long p, unsigned long long q) {
-        return (unsigned long long)__float_as_uint(fmaxf(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)q)));
-    }));
-    const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    if constexpr (EPT > 0) {
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            keep[j] = sm_exp(keep[j], base, inv_t);
-            s += keep[j];
-        }
-    } else {
-        for (size_t i = first; i < hi; i += step) {
-            load(i, keep);
-#pragma unroll
-            for (int k = 0; k < V; ++k) s += sm_exp(keep[k], base, inv_t);
-        }
-    }
-    s = __uint_as_float((uint32_t)combine(__float_as_uint(s), [](unsigned long long p, unsigned long long q) {
-        return (unsigned long long)__float_as_uint(__uint_as_float((uint32_t)p) + __uint_as_float((uint32_t)q));
-    }));
-    exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s));
-    float top = -INFINITY, sum = 0.f;
-    for (uint32_t c = 0; c < size; ++c) top = fmaxf(top, __uint_as_float((uint32_t)(xchg[c] >> 32)));
-    for (uint32_t c = 0; c < size; ++c) {
-        const float mc = __uint_as_float((uint32_t)(xchg[c] >> 32)), sc = __uint_as_float((uint32_t)xchg[c]);
-        sum += mc == -INFINITY ? sc : sc * sm_exp(mc, top, inv_t);  // (a slice of -inf has sum 0, or NaN where it holds one)
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if constexpr (EPT > 0) {
-        const float f = (m == -INFINITY ? 1.f : sm_exp(m, top, inv_t)) * inv;
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) keep[j] *= f;
-#pragma unroll
-        for (int j = 0; j < EPT / V; ++j)
-            if (first + j * step < hi) store(first + j * step, keep + j * V);
-    } else {
-        const float b = top == -INFINITY ? 0.f : top;
-        for (size_t i = first; i < hi; i += step) {
-            load(i, keep);
-#pragma unroll
-            for (int k = 0; k < V; ++k) keep[k] = sm_exp(keep[k], b, inv_t) * inv;
-            store(i, keep);
-        }
-    }
+    // A copy that a wait gave up on still writes to this memory: it has landed, or its time is long over.
+    if constexpr (AHEAD)
+        if (abort_flag) tc_warp_drain(tc_smem(&bar), turn ^ 1u);
 }
 
 // ------------------------------------------------------------------ verification of drafted tokens
@@ -218,10 +268,8 @@ struct VerifyArgs {
 
 constexpr int VF_PIECES = 1024, VF_PIECE = 512;
 
-__device__ __forceinline__ double vf_weight(double p, double q) {
-    const double w = p - q;
-    return w > 0. && w < INFINITY ? w : 0.;  // (NaN and infinities weigh nothing)
-}
+// (NaN and infinities weigh nothing; compared in 32 bits, which is exact)
+__device__ __forceinline__ double vf_weight(float p, float q) { return p > q && p < INFINITY && q > -INFINITY ? (double)p - (double)q : 0.; }
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) {
@@ -280,10 +328,10 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     struct Raw {
         uint32_t u[VEC ? 4 : 1];
     };
-    auto read = [&](const T *row, size_t i) {
+    auto read = [&](const T *row, size_t i, bool inside) {
         Raw r;
         if constexpr (VEC) {
-            if (i + V <= hi) {
+            if (inside || i + V <= hi) {
                 const uint4 q = *reinterpret_cast<const uint4 *>(row + i);
                 r.u[0] = q.x; r.u[1] = q.y; r.u[2] = q.z; r.u[3] = q.w;
             } else {
@@ -297,7 +345,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
                     }
             }
         } else {
-            r.u[0] = i < hi ? __float_as_uint(vf_f<T>(row[i])) : 0u;
+            r.u[0] = inside || i < hi ? __float_as_uint(vf_f<T>(row[i])) : 0u;
         }
         return r;
     };
@@ -312,29 +360,33 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
     auto weights = [&](size_t i, bool minus, const Raw &p, const Raw &q, double *w) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const double off = minus ? (Q ? (double)value(q, e) : (long long)(i + e) == x_held ? 1. : 0.) : 0.;
-            w[e] = vf_weight((double)value(p, e), off);
+            const float off = minus ? (Q ? value(q, e) : (long long)(i + e) == x_held ? 1.f : 0.f) : 0.f;
+            w[e] = vf_weight(value(p, e), off);
         }
     };
     auto sums = [&](bool minus) {  // of the pieces, a warp each; the CTA's total goes to everyone
         for (int j = warp; j < pieces; j += VF_THREADS / 32) {
             const size_t p0 = lo + (size_t)j * a.piece, p1 = p0 + a.piece < hi ? p0 + a.piece : hi;
             double s = 0.;
-            for (size_t i = p0 + (size_t)lane * V; i < p1; i += AHEAD * 32 * V) {
-                Raw p[AHEAD], q[AHEAD];
+            auto piece = [&](bool inside) {  // inside: no value of it lies behind the slice, so requests go out without a question each
+                for (size_t i = p0 + (size_t)lane * V; i < p1; i += AHEAD * 32 * V) {
+                    Raw p[AHEAD], q[AHEAD] = {};
 #pragma unroll
-                for (int h = 0; h < AHEAD; ++h) {
-                    p[h] = read(P, i + h * 32 * V);
-                    if (minus && Q) q[h] = read(Q, i + h * 32 * V);
+                    for (int h = 0; h < AHEAD; ++h) p[h] = read(P, i + h * 32 * V, inside);
+                    if (minus && Q)
+#pragma unroll
+                        for (int h = 0; h < AHEAD; ++h) q[h] = read(Q, i + h * 32 * V, inside);
+#pragma unroll
+                    for (int h = 0; h < AHEAD; ++h) {
+                        double w[V];
+                        weights(i + h * 32 * V, minus, p[h], q[h], w);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) s += w[e];
+                    }
                 }
-#pragma unroll
-                for (int h = 0; h < AHEAD; ++h) {
-                    double w[V];
-                    weights(i + h * 32 * V, minus, p[h], q[h], w);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) s += w[e];
-                }
-            }
+            };
+            if (p1 == p0 + a.piece) piece(true);
+            else piece(false);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             if (lane == 0) piece_sum[j] = s;
@@ -397,7 +449,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
         double w[V], mine = 0.;
 #pragma unroll
         for (int e = 0; e < V; ++e) w[e] = 0.;
-        if (i < p1) weights(i, minus, read(P, i), minus && Q ? read(Q, i) : Raw{}, w);
+        if (i < p1) weights(i, minus, read(P, i, false), minus && Q ? read(Q, i, false) : Raw{}, w);
 #pragma unroll
         for (int e = 0; e < V; ++e) mine += w[e];
         double upto = mine;
@@ -427,10 +479,11 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const VerifyArgs a) 
 // ------------------------------------------------------------------ host side
 
 template <class... KArgs>
-static int vf_launch(void (*kernel)(KArgs...), int threads, int cluster, int rows, cudaStream_t s, KArgs... args) {
+static int vf_launch(void (*kernel)(KArgs...), int threads, int cluster, int rows, size_t smem, cudaStream_t s, KArgs... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster, rows);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -438,34 +491,34 @@ static int vf_launch(void (*kernel)(KArgs...), int threads, int cluster, int row
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (smem > 48 * 1024) LCU_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     return LCU_OK;
 }
 
+template <class T, bool VEC, int EPT>
+static int softmax_ept(const SoftmaxArgs &a, int c, cudaStream_t s) {
+    // Clusters that run at once with two CTAs to an SM (15 of 16: clusters do not fill every SM), dealt evenly.
+    const int at_once = 2 * sm_count() / c * 15 / 16, turns = (a.rows + at_once - 1) / at_once, clusters = (a.rows + turns - 1) / turns;
+    if constexpr (VEC && EPT > 0)
+        if (turns > 1) return vf_launch(softmax_kernel<T, VEC, EPT, true>, SM_THREADS, c, clusters, a.slice * sizeof(T), s, (const SoftmaxArgs)a);
+    return vf_launch(softmax_kernel<T, VEC, EPT, false>, SM_THREADS, c, a.rows < 65535 ? a.rows : 65535, 0, s, (const SoftmaxArgs)a);
+}
+
 template <class T, bool VEC>
-static int softmax_launch(SoftmaxArgs a, int rows, cudaStream_t s) {
+static int softmax_launch(SoftmaxArgs a, cudaStream_t s) {
     // CTAs of a row: as many as give every thread 16 values or more
     int c = 1;
     while (c < VF_CLUSTER && a.n > (size_t)c * SM_THREADS * 16) c *= 2;
     a.slice = ((a.n + c - 1) / c + 7) / 8 * 8;
     const size_t per = (a.slice + SM_THREADS - 1) / SM_THREADS;
-    for (int r0 = 0; r0 < rows; r0 += 65535) {
-        SoftmaxArgs b = a;
-        b.probs += (size_t)r0 * a.stride_p;
-        b.logits = reinterpret_cast<const T *>(a.logits) + (size_t)r0 * a.stride_l;
-        if (b.temperature) b.temperature += r0;
-        const int m = rows - r0 < 65535 ? rows - r0 : 65535;
-        const int rc = per <= 8 ? vf_launch(softmax_kernel<T, VEC, 8>, SM_THREADS, c, m, s, (const SoftmaxArgs)b) : per <= 16 ? vf_launch(softmax_kernel<T, VEC, 16>, SM_THREADS, c, m, s, (const SoftmaxArgs)b)
-                     : per <= 32 ? vf_launch(softmax_kernel<T, VEC, 32>, SM_THREADS, c, m, s, (const SoftmaxArgs)b) : vf_launch(softmax_kernel<T, VEC, 0>, SM_THREADS, c, m, s, (const SoftmaxArgs)b);
-        if (rc) return rc;
-    }
-    return LCU_OK;
+    return per <= 8 ? softmax_ept<T, VEC, 8>(a, c, s) : per <= 16 ? softmax_ept<T, VEC, 16>(a, c, s) : per <= 32 ? softmax_ept<T, VEC, 32>(a, c, s) : softmax_ept<T, VEC, 0>(a, c, s);
 }
 
 template <class T>
-static int softmax_t(const SoftmaxArgs &a, int rows, cudaStream_t s) {
+static int softmax_t(const SoftmaxArgs &a, cudaStream_t s) {
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.probs) % 16 == 0 && a.stride_l % (16 / sizeof(T)) == 0 && a.stride_p % 4 == 0;
-    return vec ? softmax_launch<T, true>(a, rows, s) : softmax_launch<T, false>(a, rows, s);
+    return vec ? softmax_launch<T, true>(a, s) : softmax_launch<T, false>(a, s);
 }
 
 template <class T>
@@ -490,7 +543,7 @@ static int verify_t(VerifyArgs a, int n_seq, cudaStream_t s) {
         if (a.n_drafted) v.n_drafted += b0;
         v.randoms += b0 * (k + 1);
         const int m = n_seq - b0 < 65535 ? n_seq - b0 : 65535;
-        const int rc = vec ? vf_launch(verify_kernel<T, true>, VF_THREADS, c, m, s, (const VerifyArgs)v) : vf_launch(verify_kernel<T, false>, VF_THREADS, c, m, s, (const VerifyArgs)v);
+        const int rc = vec ? vf_launch(verify_kernel<T, true>, VF_THREADS, c, m, 0, s, (const VerifyArgs)v) : vf_launch(verify_kernel<T, false>, VF_THREADS, c, m, 0, s, (const VerifyArgs)v);
         if (rc) return rc;
     }
     return LCU_OK;
@@ -507,10 +560,10 @@ extern "C" int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *lo
                 n, stride_l, stride_p);
     if (rows == 0) return LCU_OK;
     LCU_REQUIRE(probs && logits, "softmax_rows: null argument");
-    const SoftmaxArgs a{probs, stride_p, logits, stride_l, temperature, n, 0};
-    if (dt == LCU_F16) return softmax_t<__half>(a, rows, as_stream(s));
-    if (dt == LCU_BF16) return softmax_t<__nv_bfloat16>(a, rows, as_stream(s));
-    return softmax_t<float>(a, rows, as_stream(s));
+    const SoftmaxArgs a{probs, stride_p, logits, stride_l, temperature, n, 0, rows};
+    if (dt == LCU_F16) return softmax_t<__half>(a, as_stream(s));
+    if (dt == LCU_BF16) return softmax_t<__nv_bfloat16>(a, as_stream(s));
+    return softmax_t<float>(a, as_stream(s));
 }
 
 extern "C" int lcu_op_verify_drafts(int32_t *accepted, int32_t *tokens, const void *target, size_t stride_t, const void *draft, size_t stride_d,

@@ -240,6 +240,23 @@ def test_the_same_answer_twice_and_on_another_stream(L):
         assert torch.equal(x.o, w)
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("nh,tokens", [(8, 1), (8, 40), (32, 33), (32, 40), (32, 100)])
+def test_slow_memory(L, dh, nh, tokens):
+    """Caches flushed ahead of each run, so that tiles of keys come late and out of step with the products: the same bits in every run.  Row tiles
+    of both kinds, prefixes that end inside a tile, several pieces of work per CTA."""
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    for prefix in (8001, 30011):
+        b = Batch(prefix + tokens, [(7, 1)] * tokens, prefix, nh, 8, dh, 1, 32)
+        first = b.run(L).clone()
+        b.check() if tokens <= 33 else None
+        for _ in range(8):
+            flush.zero_()
+            b.o.zero_()
+            b.run(L, torch.full_like(b.ws, 255))
+            assert torch.equal(b.o, first)
+
+
 def test_matches_a_contexts_own_cache(L):
     """The pages that rounds of lcu_step filled, read through lcu_kv_layer_pages and lcu_seq_pages."""
     from dataclasses import replace
