@@ -77,9 +77,9 @@ __device__ __forceinline__ void pf_arrive(uint32_t bar, int lane) {  // of a war
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pf_st32(float *p, const uint32_t *r) {  // 32 bytes, 16-byte aligned
-    reinterpret_cast<uint4 *>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
-    reinterpret_cast<uint4 *>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+__device__ __forceinline__ void pf_st32(float *p, const uint32_t *r) {  // 32 bytes at once: a row per lane, so each store is a sector of its own
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 
 // what a CTA does of one (KV head, row tile)
@@ -472,23 +472,26 @@ template <int PD> struct OwPart {
     }
 };
 
-// Adds the prefix's parts of row `row` of a KV head, normalises and stores.  Eight parts at a time, all of whose loads are in flight
-// together: rows are few next to what the memory can hold in flight, and each trip costs a microsecond.
+// Adds the prefix's parts of row `row` of a KV head, and `own` parts of its own slots in the workspace; normalises and stores.  Eight parts at a
+// time, all of whose loads are in flight together: rows are few next to what the memory can hold in flight, and each trip costs a microsecond.
 template <class T, int DH>
-__device__ __forceinline__ void ow_finish(const PrefixArgs &a, OwPart<DH / 32> &p, int hkv, int row, int lane) {
+__device__ __forceinline__ void ow_finish(const PrefixArgs &a, OwPart<DH / 32> &p, int hkv, int row, int own, int lane) {
     constexpr int PD = DH / 32, AHEAD = 8;
     const int group = a.nh / a.nkvh, tok = row / group;
     if (a.prefix_len) {
         const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, first = a.plan.first_cta(pair);
-        const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS;
-        const int parts = (int)(a.plan.last_cta(pair) - first) + 1;
+        const int shared = (int)(a.plan.last_cta(pair) - first) + 1, parts = shared + own;
+        const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS, at1 = a.own_row + (size_t)hkv * a.plan.rows + row;
+        const size_t apart1 = (size_t)a.nkvh * a.plan.rows;
+        auto at = [&](int s) { return s < shared ? at0 + (size_t)s * a.plan.slot_rows : at1 + (size_t)(s - shared) * apart1; };
 #pragma unroll 1
         for (int s0 = 0; s0 < parts; s0 += AHEAD) {
             float v[AHEAD][PD];
-            const float2 x = lane < AHEAD && s0 + lane < parts ? __ldcg(a.part_ml + at0 + (size_t)(s0 + lane) * a.plan.slot_rows) : make_float2(-INFINITY, 0.f);
+            const float2 x = lane < AHEAD && s0 + lane < parts ? __ldcg(a.part_ml + at(s0 + lane)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                const float *src = a.part_o + (at0 + (size_t)min(s0 + i, parts - 1) * a.plan.slot_rows) * DH;
+                if (s0 + i >= parts) break;
+                const float *src = a.part_o + at(s0 + i) * DH;
                 if constexpr (PD == 4) {
                     const float4 y = __ldcg(reinterpret_cast<const float4 *>(src) + lane);
                     v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
@@ -735,7 +738,7 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
             OwPart<PD> p;
             p.clear();
             for (int s = 0; s < splits; ++s) p.add(cluster_ml[(s * 16 + r) * 2], cluster_ml[(s * 16 + r) * 2 + 1], cluster_o + ((size_t)s * 16 + r) * DH + lane * PD);
-            ow_finish<T, DH>(a, p, hkv, t * group + r, lane);
+            ow_finish<T, DH>(a, p, hkv, t * group + r, 0, lane);
         }
         return;
     }
@@ -755,13 +758,13 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
 #pragma unroll 1
     for (int r = warp; r < rows; r += OW_WARPS) {
         OwPart<PD> p = both(r);
-        ow_finish<T, DH>(a, p, hkv, t * group + r, lane);
+        ow_finish<T, DH>(a, p, hkv, t * group + r, 0, lane);
     }
 }
 
 // Sum of a row's own part and the prefix's: a warp per row, behind own_kernel (which ends behind the prefix).
 template <class T, int DH>
-__global__ void __launch_bounds__(256) own_sum_kernel(const PrefixArgs a, int splits) {
+__global__ void __launch_bounds__(256, 4) own_sum_kernel(const PrefixArgs a, int splits) {
     constexpr int PD = DH / 32;
     const int lane = threadIdx.x & 31, hkv = blockIdx.y, row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= a.plan.rows) return;
@@ -770,19 +773,7 @@ __global__ void __launch_bounds__(256) own_sum_kernel(const PrefixArgs a, int sp
     grid_dep_wait();
     OwPart<PD> p;
     p.clear();
-    for (int i = 0; i < splits; ++i) {
-        const size_t at = a.own_row + ((size_t)i * a.nkvh + hkv) * a.plan.rows + row;
-        const float2 x = __ldcg(a.part_ml + at);
-        float v[PD];
-#pragma unroll
-        for (int d = 0; d < PD; d += 2) {
-            const float2 y = __ldcg(reinterpret_cast<const float2 *>(a.part_o + at * DH + lane * PD + d));
-            v[d] = y.x;
-            v[d + 1] = y.y;
-        }
-        p.add(x.x, x.y, v);
-    }
-    ow_finish<T, DH>(a, p, hkv, row, lane);
+    ow_finish<T, DH>(a, p, hkv, row, splits, lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -851,7 +842,7 @@ using namespace lcu;
 
 extern "C" size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len) {
     if (n <= 0 || nkvh <= 0 || nh < nkvh || nh % nkvh || dh <= 0 || !prefix_len) return 0;
-    return prefix_bytes(prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count()), nkvh, dh);
+    return prefix_bytes(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh);
 }
 
 extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q, int stq, int shq, const lcu_kv_pages *pages, const int32_t *prefix_table,
@@ -882,7 +873,7 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
     a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale * 1.4426950408889634f;
     if (prefix_len) {
-        a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count());
+        a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh, (long long)(n_seq < n ? n_seq : n) * table_stride * pages->page_tokens);
         a.part_ml = reinterpret_cast<float2 *>(workspace);
         a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan, nkvh));
         a.own_row = prefix_own_row(a.plan);

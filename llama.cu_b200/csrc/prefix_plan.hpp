@@ -23,7 +23,7 @@ struct PrefixPlan {
     int ctas;
     int slot_rows;   // rows of a piece's slot
     // More (KV head, token) blocks for the own slots than SMs: they leave their parts too, at most so many of a row, and a kernel of its
-    // own adds up.  (A block that adds up waits for the prefix, and would hold its place beside it from the blocks that have not begun.)
+    // own adds up.  (A block that adds up waits for the prefix, and would hold its place from the blocks that have not begun.)  0: none.
     int own_parts;
 
     LCU_HD long long first_cta(long long pair) const { return pair * key_tiles / per; }
@@ -31,26 +31,53 @@ struct PrefixPlan {
     LCU_HD long long slots() const { return ctas + pairs; }
 };
 
-// n tokens, `group` query heads per KV head, a prefix of prefix_len > 0 positions, at most `sms` CTAs
-inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, int sms) {
+// Number of (KV head, row tile) pairs of n tokens, `group` query heads per KV head; parts of a row's own slots.
+inline long long prefix_pairs(int n, int group, int nkvh) { return (long long)nkvh * ((n * group + PF_ROWS - 1) / PF_ROWS); }
+inline int prefix_own_parts(int n, int nkvh, int sms) {
+    const long long blocks = (long long)n * nkvh;
+    return blocks <= sms ? 0 : blocks >= 12LL * sms ? 1 : (int)(12LL * sms / blocks);
+}
+
+// A prefix of prefix_len > 0 positions, at most `sms` CTAs; own_slots: what the sequences' own tables have room for.
+// One CTA of the prefix fills an SM.  The own slots' blocks get the SMs that it leaves, and all of them behind it: fewer CTAs of the prefix
+// with more key tiles each make it longer and the rest shorter.  Estimates in microseconds: 8 to begin and end, a key tile 1.2 to 2.4 (heads
+// of 0 to 128), 7 from a piece to the next, own slots (half of what there is room for) at 30 KB per SM.
+inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, int sms, int dh, long long own_slots) {
     PrefixPlan p;
     p.rows = n * group;
     p.row_tiles = (p.rows + PF_ROWS - 1) / PF_ROWS;
     p.key_tiles = (int)((prefix_len + PF_TILE - 1) / PF_TILE);
-    p.pairs = (long long)nkvh * p.row_tiles;
+    p.pairs = prefix_pairs(n, group, nkvh);
     p.units = p.pairs * p.key_tiles;
-    p.per = (p.units + sms - 1) / sms;
-    p.ctas = (int)((p.units + p.per - 1) / p.per);
     p.slot_rows = p.rows < PF_ROWS ? p.rows : PF_ROWS;
-    const long long blocks = (long long)n * nkvh;
-    p.own_parts = blocks <= sms ? 0 : blocks >= 6LL * sms ? 1 : (int)(6LL * sms / blocks);
+    p.own_parts = prefix_own_parts(n, nkvh, sms);
+    const double tile = 1.2 + 1.2 * dh / 128, own = (double)nkvh * own_slots * dh * 4 * 0.5 / 30e3;  // the latter in SM microseconds
+    const long long least = (p.units + sms - 1) / sms;
+    double best = 0;
+    for (long long per = least; per <= 8 * least && per <= p.units; ++per) {
+        const long long ctas = (p.units + per - 1) / per;
+        const long long pieces = per >= p.key_tiles ? (per + p.key_tiles - 1) / p.key_tiles : p.key_tiles % per ? 2 : 1;
+        const double prefix = 1 + 7 * pieces + tile * per, left = p.own_parts ? own - (double)(sms - ctas) * (prefix - 8) : 0;
+        const double t = prefix + (left > 0 ? left / sms + (left < 4.0 * sms ? left * 1.5 / sms : 6) : 0);
+        if (per == least || t < best) {
+            best = t;
+            p.per = per;
+            p.ctas = (int)ctas;
+        }
+        if (!p.own_parts || per > least + 64) break;
+    }
     return p;
 }
 
-// Workspace, in rows: those of every slot, then those of the own parts, [part][KV head][row].  (maximum, sum) of each, then their unnormalised outputs.
+// Workspace: (maximum, sum) of each row of every slot, then of the own parts, [part][KV head][row]; then their unnormalised outputs.
 inline size_t prefix_own_row(const PrefixPlan &p) { return (size_t)p.slots() * p.slot_rows; }
 inline size_t prefix_part_rows(const PrefixPlan &p, int nkvh) { return prefix_own_row(p) + (size_t)p.own_parts * nkvh * p.rows; }
 inline size_t prefix_ml_bytes(const PrefixPlan &p, int nkvh) { return (prefix_part_rows(p, nkvh) * 8 + 255) / 256 * 256; }
-inline size_t prefix_bytes(const PrefixPlan &p, int nkvh, int dh) { return prefix_ml_bytes(p, nkvh) + prefix_part_rows(p, nkvh) * dh * 4; }
+// ... at most, whatever the plan
+inline size_t prefix_bytes(int n, int group, int nkvh, uint32_t prefix_len, int sms, int dh) {
+    PrefixPlan p = prefix_plan(n, group, nkvh, prefix_len, sms, dh, 0);
+    p.ctas = sms;
+    return prefix_ml_bytes(p, nkvh) + prefix_part_rows(p, nkvh) * dh * 4;
+}
 
 }  // namespace lcu
