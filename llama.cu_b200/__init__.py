@@ -263,8 +263,10 @@ def ptr(t):
 
 def stream_ptr(stream=None):
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without the Stream object that current_stream() builds (3.5 of a call's 10 us)
+    return C.c_void_p(raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream)
 
 
 TORCH_DT = None

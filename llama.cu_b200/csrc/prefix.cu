@@ -792,12 +792,18 @@ static int pf_map(CUtensorMap *m, int dt, const void *base, const lcu_kv_pages &
 
 template <class T, int DH>
 static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
+    static OncePerDevice once;
+    const int set = once.run([]() -> int {
+        LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem<DH>()));
+        LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>() + 8 * ow_part_bytes<DH>())));
+        return LCU_OK;
+    });
+    if (set) return set;
     if (a.prefix_len) {
         CUtensorMap mk, mv;
         int rc = pf_map(&mk, dt, a.pages.k, a.pages, DH, a.nkvh);
         if (!rc) rc = pf_map(&mv, dt, a.pages.v, a.pages, DH, a.nkvh);
         if (rc) return rc;
-        LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem<DH>()));
         LCU_CHECK_CUDA(launch_kernel(prefix_tc_kernel<T, DH>, dim3(a.plan.ctas), dim3(PF_THREADS), pf_smem<DH>(), s, false, a, mk, mv, dt == LCU_BF16 ? 1u : 0u));
     }
     const int group = a.nh / a.nkvh, tokens_per = 16 / group;
@@ -808,9 +814,6 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
     if (leave) splits = (int)(cap < 64LL * a.plan.own_parts ? (cap + 63) / 64 > 0 ? (cap + 63) / 64 : 1 : a.plan.own_parts);
     else while (splits < 8 && blocks * splits <= sm_count() && cap > (long long)splits * 64) splits *= 2;
     const size_t smem = ow_smem<DH>() + (splits > 1 && !leave ? splits * ow_part_bytes<DH>() : 0);
-    LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>() + 8 * ow_part_bytes<DH>())));
-    LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.nkvh, a.n);
     cfg.blockDim = dim3(OW_THREADS);

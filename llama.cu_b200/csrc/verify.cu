@@ -1,10 +1,11 @@
 // From logits to the tokens that a verified draft leaves (no counterpart in the reference, which samples one token per row,
 // exec/output_head.rs:104-113): probabilities of rows of logits, and the acceptance of drafted tokens against them.
+#include "paged.cuh"
 #include "tc.cuh"
 
 namespace lcu {
 
-constexpr int VF_THREADS = 256, SM_THREADS = 512;
+constexpr int VF_THREADS = 256;
 constexpr int VF_CLUSTER = 8;
 
 __device__ __forceinline__ void vf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -33,24 +34,40 @@ template <> __device__ __forceinline__ float vf_f<float>(float v) { return v; }
 //   p_j = exp((x_j - m) / T) / sum_i exp((x_i - m) / T),   m the largest;   T = 0: 1 at the lowest index of the largest, 0 elsewhere
 //
 // Bound by HBM: a row is read once and written once.  A thread-block cluster of up to 8 CTAs takes a row and keeps its values in
-// registers between the two halves (vocabularies up to 131072; longer rows are read a second time, from L2); maxima and sums, relative
+// registers between the two halves (vocabularies up to 262144; longer rows are read a second time, from L2); maxima and sums, relative
 // to each CTA's own maximum, cross the cluster as pairs in one exchange.  Where there are more rows than clusters at once, clusters stay and each
 // CTA requests its part of the next row (one bulk copy into shared memory) as soon as it has taken up this one: the memory works on
 // while maxima, exponentials and sums wait for one another.
+//
+// Rows of any stride: where the strides of logits and probabilities agree modulo a 16-byte piece, a row is taken from the piece on that it begins
+// in, and what lies ahead of it in that piece counts as -inf and is not written.
 struct SoftmaxArgs {
     float *probs;
     size_t stride_p;
     const void *logits;
     size_t stride_l;
     const float *temperature;
-    size_t n, slice;  // values of a row, of a CTA
-    int rows;
+    uint32_t n, slice;  // values of a row, of a CTA
+    int rows, wide;     // wide: pieces of eight probabilities begin on 32 bytes
 };
 
-// 2^((x - m) c), c = log2(e) / T: the difference first, so that what is rounded shrinks with it; off by 2^-22 and 3 |z| 2^-24 relatively
-__device__ __forceinline__ float sm_exp(float x, float m, float c) {
+// 2^v; NARROW: v >= -126, where no result is subnormal (without the scaling that those need: three instructions of eight)
+template <bool NARROW> __device__ __forceinline__ float sm_exp2(float v) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"((x - m) * c));
+    if (NARROW) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    else asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// 2^((x - m) c), c = log2(e) / T: the difference first, so that what is rounded shrinks with it; off by 2^-22 and 3 |z| 2^-24 relatively
+__device__ __forceinline__ float sm_exp(float x, float m, float c) { return sm_exp2<false>((x - m) * c); }
+__device__ __forceinline__ float sm_max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+__device__ __forceinline__ float sm_min3(float x, float y, float z) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
 
@@ -62,12 +79,15 @@ __device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
     return ((unsigned long long)u << 32) | (uint32_t)~i;
 }
 
-// grid (CTAs of a cluster, clusters)
-template <class T, bool VEC, int EPT, bool AHEAD>
-__global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArgs a) {
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+// grid (CTAs of a cluster, clusters); V values to a piece (1: rows are not in pieces of 16 bytes)
+template <class T, int V, int NT, int EPT, bool AHEAD>
+__global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArgs a) {
+    constexpr uint32_t STEP = NT * V;
+    constexpr int WARPS = NT / 32;
     extern __shared__ __align__(16) unsigned char staged[];  // AHEAD: this CTA's part of the next row
-    __shared__ unsigned long long part[SM_THREADS / 32], xchg[2][VF_CLUSTER], xbar[2], bar;
+    __shared__ unsigned long long part[WARPS], xchg[2][VF_CLUSTER], xbar[2], bar;
+    __shared__ float2 fpart[WARPS];
+    __shared__ float spart[WARPS];
     __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = vf_rank(), size = gridDim.x;
@@ -80,31 +100,31 @@ __global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArg
     }
     __syncthreads();
     vf_cluster_arrive();  // waited for ahead of the first exchange: a peer's shared memory is there once it runs, its barriers once it arrives
-    const size_t lo = (size_t)rank * a.slice < a.n ? (size_t)rank * a.slice : a.n, hi = lo + a.slice < a.n ? lo + a.slice : a.n;
-    const size_t whole = AHEAD ? lo + (hi - lo) / V * V : lo;  // values below it come through shared memory
     const T *base = reinterpret_cast<const T *>(a.logits);
-    auto request = [&](int row) {
-        const uint32_t bytes = (uint32_t)((whole - lo) * sizeof(T));
-        if (!AHEAD || tid != 0 || bytes == 0 || row >= a.rows) return;
+    const float nan = __int_as_float(0x7fc00000);
+    // Places of a row are counted from the piece that it begins in: its values are skip .. skip + n.
+    auto skip_of = [&](int row) { return V > 1 ? (uint32_t)((size_t)row * a.stride_l % V) : 0u; };
+    auto range = [&](uint32_t skip, uint32_t &lo, uint32_t &hi) {
+        const unsigned long long end = (unsigned long long)a.n + skip, from = (unsigned long long)rank * a.slice;
+        lo = (uint32_t)(from < end ? from : end);
+        hi = (uint32_t)(from + a.slice < end ? from + a.slice : end);
+    };
+    auto bytes_ahead = [&](uint32_t lo, uint32_t hi) { return (hi - lo) / V * V * (uint32_t)sizeof(T); };
+    auto request = [&](int row) {  // whole pieces of the slice
+        if (!AHEAD || tid != 0 || row >= a.rows) return;
+        const uint32_t skip = skip_of(row);
+        uint32_t lo, hi;
+        range(skip, lo, hi);
+        const uint32_t bytes = bytes_ahead(lo, hi);
+        if (bytes == 0) return;
         tc_mbar_expect_tx(tc_smem(&bar), bytes);
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                     ::"r"(tc_smem(staged)), "l"(base + (size_t)row * a.stride_l + lo), "r"(bytes), "r"(tc_smem(&bar)) : "memory");
+                     ::"r"(tc_smem(staged)), "l"(base + (size_t)row * a.stride_l - skip + lo), "r"(bytes), "r"(tc_smem(&bar)) : "memory");
     };
     request(blockIdx.y);
-    auto combine = [&](unsigned long long v, auto op) {  // over the block
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-        if (lane == 0) part[warp] = v;
-        __syncthreads();
-        v = part[lane % (SM_THREADS / 32)];
-#pragma unroll
-        for (int o = SM_THREADS / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-        __syncthreads();
-        return v;
-    };
     // Into everyone's slots, in turns.  A peer writes a turn's slots again only two rows on, and by then it has had this CTA's value of the row
     // between, which is sent behind the last read of these.
-    uint32_t turn = 0, phase = 0;
+    uint32_t turn = 0, phase = 0, bar_phase = 0;
     bool begun = false;
     auto exchange = [&](unsigned long long v) {
         if (!begun) vf_cluster_wait();
@@ -115,21 +135,25 @@ __global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArg
         if (!ok) abort_flag = 1;
         return ok;
     };
-    auto greater = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
-    const size_t first = lo + (size_t)tid * V;
-    constexpr size_t step = (size_t)SM_THREADS * V;
 
     for (int row = blockIdx.y; row < a.rows; row += gridDim.y, phase ^= turn, turn ^= 1u) {
-        const T *x = base + (size_t)row * a.stride_l;
-        float *out = a.probs + (size_t)row * a.stride_p;
+        const uint32_t skip = skip_of(row);
+        uint32_t lo, hi;
+        range(skip, lo, hi);
+        const T *x = base + (size_t)row * a.stride_l - skip;
+        float *out = a.probs + (size_t)row * a.stride_p - skip;
         const float t = a.temperature ? a.temperature[row] : 1.f;
         const float inv_t = 1.f / t > 2.0e38f ? 2.0e38f * 1.442695041f : 1.442695041f / t;  // finite: (x - m) / T stays 0 where x = m, however small T
         bool here = true;
-        if constexpr (AHEAD) here = whole == lo || tc_mbar_wait(tc_smem(&bar), turn, &abort_flag);
-        if (!here) abort_flag = 1;
-        auto load = [&](size_t i, float *f) {  // V values from i on; -inf behind the slice
-            if (VEC && i + V <= hi) {
-                const uint4 q = AHEAD ? *reinterpret_cast<const uint4 *>(staged + (i - lo) * sizeof(T)) : *reinterpret_cast<const uint4 *>(x + i);
+        if (AHEAD && bytes_ahead(lo, hi)) {
+            here = tc_mbar_wait(tc_smem(&bar), bar_phase, &abort_flag);
+            if (!here) abort_flag = 1;
+            bar_phase ^= 1u;
+        }
+        const uint32_t first = lo + tid * V;
+        auto load = [&](uint32_t i, float *f) {  // V values from place i on; -inf outside the row's part of the slice
+            if (V > 1 && i >= skip && i + V <= hi) {
+                const uint4 q = AHEAD ? *reinterpret_cast<const uint4 *>(staged + (i - lo) * (uint32_t)sizeof(T)) : *reinterpret_cast<const uint4 *>(x + i);
                 const uint32_t w[4] = {q.x, q.y, q.z, q.w};
                 if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -139,90 +163,133 @@ __global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArg
                     for (int k = 0; k < V; k += 2) {
                         const float2 p = Act<T>::to_f2(w[k / 2]);
                         f[k] = p.x;
-                        f[k + 1] = p.y;
+                        if (V > 1) f[k + 1] = p.y;
                     }
                 }
                 return;
             }
 #pragma unroll
-            for (int k = 0; k < V; ++k) f[k] = i + k < hi ? vf_f<T>(x[i + k]) : -INFINITY;
+            for (int k = 0; k < V; ++k) f[k] = i + k >= skip && i + k < hi ? vf_f<T>(x[i + k]) : -INFINITY;
         };
-        auto store = [&](size_t i, const float *f) {
-            if (VEC && i + V <= hi) {
+        auto store = [&](uint32_t i, const float *f) {
+            if (V > 1 && i >= skip && i + V <= hi) {
+                if (V == 8 && a.wide) {  // a sector at once, not its halves
+                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                                 ::"l"(out + i), "f"(f[0]), "f"(f[1 % V]), "f"(f[2 % V]), "f"(f[3 % V]), "f"(f[4 % V]), "f"(f[5 % V]), "f"(f[6 % V]), "f"(f[7 % V]) : "memory");
+                    return;
+                }
 #pragma unroll
-                for (int k = 0; k < V; k += 4) __stcs(reinterpret_cast<float4 *>(out + i + k), make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]));
+                for (int k = 0; k < V; k += 4) __stcs(reinterpret_cast<float4 *>(out + i + k), make_float4(f[k], f[k + 1 < V ? k + 1 : 0], f[k + 2 < V ? k + 2 : 0], f[k + 3 < V ? k + 3 : 0]));
                 return;
             }
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (i + k < hi) __stcs(out + i + k, f[k]);
+                if (i + k >= skip && i + k < hi) __stcs(out + i + k, f[k]);
         };
         float keep[EPT > 0 ? EPT : V];
         if (t == 0.f) {  // (uniform over the cluster)
             unsigned long long best = 0;
-            for (size_t i = first; i < hi; i += step) {
+            for (uint32_t i = first; i < hi; i += STEP) {
                 load(i, keep);
 #pragma unroll
                 for (int k = 0; k < V; ++k)
-                    if (i + k < hi) best = greater(best, sm_key(keep[k], (uint32_t)(i + k)));
+                    if (i + k >= skip && i + k < hi) {
+                        const unsigned long long key = sm_key(keep[k], i + k);
+                        best = best > key ? best : key;
+                    }
             }
-            best = combine(best, greater);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const unsigned long long v = __shfl_xor_sync(0xffffffffu, best, o);
+                best = best > v ? best : v;
+            }
+            if (lane == 0) part[warp] = best;
+            __syncthreads();
             request(row + gridDim.y);
+            for (int w = 0; w < WARPS; ++w) best = best > part[w] ? best : part[w];
             here = exchange(best) && here;
             best = 0;
-            for (uint32_t c = 0; c < size; ++c) best = greater(best, xchg[turn][c]);
+            for (uint32_t c = 0; c < size; ++c) best = best > xchg[turn][c] ? best : xchg[turn][c];
             // a row of -inf (and NaN) alone has no largest
-            const bool some = (uint32_t)(best >> 32) > 0x007fffffu;
-            const size_t at = some ? (size_t)(uint32_t)~(uint32_t)best : a.n;
-            for (size_t i = first; i < hi; i += step) {
+            const uint32_t at = (uint32_t)(best >> 32) > 0x007fffffu ? (uint32_t)~(uint32_t)best : 0xffffffffu;
+            for (uint32_t i = first; i < hi; i += STEP) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) keep[k] = !here ? __int_as_float(0x7fc00000) : i + k == at ? 1.f : 0.f;
+                for (int k = 0; k < V; ++k) keep[k] = !here ? nan : i + k == at ? 1.f : 0.f;
                 store(i, keep);
             }
+            __syncthreads();  // part has been read
             continue;
         }
-        float m = -INFINITY;
+        float m = -INFINITY, low = INFINITY;  // the largest, the smallest
+        auto extend = [&](const float *f, int count) {
+            if (V == 1) {
+#pragma unroll
+                for (int k = 0; k < count; ++k) m = fmaxf(m, f[k]), low = fminf(low, f[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < count; k += 2) m = sm_max3(m, f[k], f[k + 1]), low = sm_min3(low, f[k], f[k + 1]);
+            }
+        };
         if constexpr (EPT > 0) {
 #pragma unroll
-            for (int j = 0; j < EPT / V; ++j) load(first + j * step, keep + j * V);
-            if (AHEAD && !here) keep[0] = __int_as_float(0x7fc00000);  // the copy never came: the row becomes NaN
+            for (int j = 0; j < EPT / V; ++j) load(first + j * STEP, keep + j * V);
+            if (AHEAD && !here) keep[0] = nan;  // the copy never came: the row becomes NaN
 #pragma unroll
-            for (int j = 0; j < EPT; ++j) m = fmaxf(m, keep[j]);
+            for (int j = 0; j < EPT / V; ++j)
+                if (first + j * STEP < hi) extend(keep + j * V, V);
         } else {
-            for (size_t i = first; i < hi; i += step) {
+            for (uint32_t i = first; i < hi; i += STEP) {
                 load(i, keep);
-#pragma unroll
-                for (int k = 0; k < V; ++k) m = fmaxf(m, keep[k]);
+                extend(keep, V);
             }
         }
-        m = __uint_as_float((uint32_t)combine(__float_as_uint(m), [](unsigned long long p, unsigned long long q) {
-            return (unsigned long long)__float_as_uint(fmaxf(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)q)));
-        }));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o)), low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        if (lane == 0) fpart[warp] = make_float2(m, low);
+        __syncthreads();
         request(row + gridDim.y);  // everyone has taken this row up
+        {
+            const float2 v = fpart[lane % WARPS];
+            m = v.x;
+            low = v.y;
+        }
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o)), low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         const float off = m == -INFINITY ? 0.f : m;
         float s = 0.f;
         if constexpr (EPT > 0) {
+            if ((low - off) * inv_t >= -126.f) {  // (the block's smallest: one way for all its threads)
 #pragma unroll
-            for (int j = 0; j < EPT; ++j) {
-                keep[j] = sm_exp(keep[j], off, inv_t);
-                s += keep[j];
+                for (int j = 0; j < EPT; ++j) s += keep[j] = sm_exp2<true>((keep[j] - off) * inv_t);
+            } else {
+#pragma unroll
+                for (int j = 0; j < EPT; ++j) s += keep[j] = sm_exp2<false>((keep[j] - off) * inv_t);
             }
         } else {
-            for (size_t i = first; i < hi; i += step) {
+            for (uint32_t i = first; i < hi; i += STEP) {
                 load(i, keep);
 #pragma unroll
                 for (int k = 0; k < V; ++k) s += sm_exp(keep[k], off, inv_t);
             }
         }
-        s = __uint_as_float((uint32_t)combine(__float_as_uint(s), [](unsigned long long p, unsigned long long q) {
-            return (unsigned long long)__float_as_uint(__uint_as_float((uint32_t)p) + __uint_as_float((uint32_t)q));
-        }));
-        if (!exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s))) s = __int_as_float(0x7fc00000);
-        float top = -INFINITY, sum = 0.f;
-        for (uint32_t c = 0; c < size; ++c) top = fmaxf(top, __uint_as_float((uint32_t)(xchg[turn][c] >> 32)));
-        for (uint32_t c = 0; c < size; ++c) {
-            const float mc = __uint_as_float((uint32_t)(xchg[turn][c] >> 32)), sc = __uint_as_float((uint32_t)xchg[turn][c]);
-            sum += mc == -INFINITY ? sc : sc * sm_exp(mc, top, inv_t);  // (a slice of -inf has sum 0, or NaN where it holds one)
+        s = warp_sum(s);
+        if (lane == 0) spart[warp] = s;
+        __syncthreads();
+        s = spart[lane % WARPS];
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (!exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s))) s = nan;
+        float top, sum;
+        {  // a CTA's pair per lane
+            const unsigned long long v = xchg[turn][lane % VF_CLUSTER < size ? lane % VF_CLUSTER : 0];
+            const bool one = lane % VF_CLUSTER < size;
+            const float mc = __uint_as_float((uint32_t)(v >> 32)), sc = __uint_as_float((uint32_t)v);
+            top = mc;
+#pragma unroll
+            for (int o = VF_CLUSTER / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            sum = !one ? 0.f : mc == -INFINITY ? sc : sc * sm_exp(mc, top, inv_t);  // (a slice of -inf has sum 0, or NaN where it holds one)
+#pragma unroll
+            for (int o = VF_CLUSTER / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
         const float inv = sum == 0.f ? 0.f : s != s ? s : 1.f / sum;  // (NaN among this CTA's values, or a peer that never came)
         if constexpr (EPT > 0) {
@@ -231,10 +298,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArg
             for (int j = 0; j < EPT; ++j) keep[j] *= f;
 #pragma unroll
             for (int j = 0; j < EPT / V; ++j)
-                if (first + j * step < hi) store(first + j * step, keep + j * V);
+                if (first + j * STEP < hi) store(first + j * STEP, keep + j * V);
         } else {
             const float b = top == -INFINITY ? 0.f : top;
-            for (size_t i = first; i < hi; i += step) {
+            for (uint32_t i = first; i < hi; i += STEP) {
                 load(i, keep);
 #pragma unroll
                 for (int k = 0; k < V; ++k) keep[k] = sm_exp(keep[k], b, inv_t) * inv;
@@ -244,7 +311,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) softmax_kernel(const SoftmaxArg
     }
     // A copy that a wait gave up on still writes to this memory: it has landed, or its time is long over.
     if constexpr (AHEAD)
-        if (abort_flag) tc_warp_drain(tc_smem(&bar), turn ^ 1u);
+        if (abort_flag) tc_warp_drain(tc_smem(&bar), bar_phase ^ 1u);
 }
 
 // ------------------------------------------------------------------ verification of drafted tokens
@@ -491,34 +558,50 @@ static int vf_launch(void (*kernel)(KArgs...), int threads, int cluster, int row
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (smem > 48 * 1024) LCU_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     return LCU_OK;
 }
 
-template <class T, bool VEC, int EPT>
+template <class T, int V, int NT, int EPT>
 static int softmax_ept(const SoftmaxArgs &a, int c, cudaStream_t s) {
-    // Clusters that run at once with two CTAs to an SM (15 of 16: clusters do not fill every SM), dealt evenly.
-    const int at_once = 2 * sm_count() / c * 15 / 16, turns = (a.rows + at_once - 1) / at_once, clusters = (a.rows + turns - 1) / turns;
-    if constexpr (VEC && EPT > 0)
-        if (turns > 1) return vf_launch(softmax_kernel<T, VEC, EPT, true>, SM_THREADS, c, clusters, a.slice * sizeof(T), s, (const SoftmaxArgs)a);
-    return vf_launch(softmax_kernel<T, VEC, EPT, false>, SM_THREADS, c, a.rows < 65535 ? a.rows : 65535, 0, s, (const SoftmaxArgs)a);
+    // Clusters that run at once with 1024 threads to an SM (15 of 16: clusters do not fill every SM), dealt evenly.
+    const int at_once = 1024 / NT * sm_count() / c * 15 / 16, turns = (a.rows + at_once - 1) / at_once, clusters = (a.rows + turns - 1) / turns;
+    if constexpr (V > 1 && EPT > 0)
+        if (turns > 1) {
+            static OncePerDevice once;
+            const int set = once.run([]() -> int {
+                LCU_CHECK_CUDA(cudaFuncSetAttribute(softmax_kernel<T, V, NT, EPT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, NT * EPT * (int)sizeof(T)));
+                return LCU_OK;
+            });
+            if (set) return set;
+            return vf_launch(softmax_kernel<T, V, NT, EPT, true>, NT, c, clusters, (size_t)a.slice * sizeof(T), s, (const SoftmaxArgs)a);
+        }
+    return vf_launch(softmax_kernel<T, V, NT, EPT, false>, NT, c, a.rows < 65535 ? a.rows : 65535, 0, s, (const SoftmaxArgs)a);
 }
 
-template <class T, bool VEC>
+// Threads hold up to 32 values, and 8 CTAs a row: of 256 threads where that is enough (the waits of a row, for its values, twice for the
+// block, for the cluster, are then shared by more rows), of 512 or 1024 for vocabularies of up to 262144.  As few CTAs to a row as hold it
+// where rows fill the SMs (1000 rows of 20000: 51 us with 8, 42 with 4), more where they do not.
+template <class T, int V>
 static int softmax_launch(SoftmaxArgs a, cudaStream_t s) {
-    // CTAs of a row: as many as give every thread 16 values or more
+    const uint32_t most = a.n + (a.rows > 1 && a.stride_l % V ? V - 1 : 0);  // places of a row
+    const uint32_t threads = most <= 256u * 32 * VF_CLUSTER ? 256 : most <= 512u * 32 * VF_CLUSTER ? 512 : 1024;
     int c = 1;
-    while (c < VF_CLUSTER && a.n > (size_t)c * SM_THREADS * 16) c *= 2;
-    a.slice = ((a.n + c - 1) / c + 7) / 8 * 8;
-    const size_t per = (a.slice + SM_THREADS - 1) / SM_THREADS;
-    return per <= 8 ? softmax_ept<T, VEC, 8>(a, c, s) : per <= 16 ? softmax_ept<T, VEC, 16>(a, c, s) : per <= 32 ? softmax_ept<T, VEC, 32>(a, c, s) : softmax_ept<T, VEC, 0>(a, c, s);
+    while (c < VF_CLUSTER && most > (size_t)c * threads * 32) c *= 2;
+    while (c < VF_CLUSTER && (long long)a.rows * c * 2 <= 1024 / (int)threads * sm_count() && most > (size_t)c * threads * 8) c *= 2;
+    a.slice = (most + c - 1) / c;
+    a.slice = (a.slice + 7) / 8 * 8;
+    const uint32_t per = (a.slice + threads - 1) / threads;
+    if (threads == 256) return per <= 8 ? softmax_ept<T, V, 256, 8>(a, c, s) : per <= 16 ? softmax_ept<T, V, 256, 16>(a, c, s) : softmax_ept<T, V, 256, 32>(a, c, s);
+    if (threads == 512) return softmax_ept<T, V, 512, 32>(a, c, s);
+    return per <= 32 ? softmax_ept<T, V, 1024, 32>(a, c, s) : softmax_ept<T, V, 512, 0>(a, c, s);
 }
 
 template <class T>
 static int softmax_t(const SoftmaxArgs &a, cudaStream_t s) {
-    const bool vec = ((uintptr_t)a.logits | (uintptr_t)a.probs) % 16 == 0 && a.stride_l % (16 / sizeof(T)) == 0 && a.stride_p % 4 == 0;
-    return vec ? softmax_launch<T, true>(a, s) : softmax_launch<T, false>(a, s);
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool pieces = ((uintptr_t)a.logits | (uintptr_t)a.probs) % 16 == 0 && (a.rows == 1 || a.stride_l % V == a.stride_p % V);
+    return pieces ? softmax_launch<T, V>(a, s) : softmax_launch<T, 1>(a, s);
 }
 
 template <class T>
@@ -560,7 +643,7 @@ extern "C" int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *lo
                 n, stride_l, stride_p);
     if (rows == 0) return LCU_OK;
     LCU_REQUIRE(probs && logits, "softmax_rows: null argument");
-    const SoftmaxArgs a{probs, stride_p, logits, stride_l, temperature, n, 0, rows};
+    const SoftmaxArgs a{probs, stride_p, logits, stride_l, temperature, (uint32_t)n, 0, rows, (uintptr_t)probs % 32 == 0};
     if (dt == LCU_F16) return softmax_t<__half>(a, as_stream(s));
     if (dt == LCU_BF16) return softmax_t<__nv_bfloat16>(a, as_stream(s));
     return softmax_t<float>(a, as_stream(s));
