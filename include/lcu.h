@@ -541,7 +541,8 @@ typedef struct {
 LCU_API int lcu_kv_layer_pages(const lcu_ctx *ctx, int layer, lcu_kv_pages *out);
 LCU_API int lcu_seq_pages(const lcu_ctx *ctx, int seq, int32_t *ids, int cap, int *n_out);
 /* Queries [n, nh, dh] and keys [n, nkvh, dh] in one pass (nh or nkvh may be 0), dh <= 256, dt LCU_F16, LCU_BF16 or LCU_F32.  Outputs may be
- * the inputs (same strides), and may not overlap them otherwise.  A token whose position is not below n_pos is left unwritten. */
+ * the inputs (same strides), and may not overlap them otherwise.  A token whose position is not below n_pos is left unwritten (pos may be
+ * NULL when rot_dims == 0).  n up to 2^30. */
 LCU_API int lcu_op_qk_norm_rope(void *q_out, int stride_tok_qo, int stride_head_qo, const void *q, int stride_tok_q, int stride_head_q, void *k_out,
                                 int stride_tok_ko, int stride_head_ko, const void *k, int stride_tok_k, int stride_head_k, const uint32_t *pos,
                                 const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s);
@@ -569,9 +570,10 @@ LCU_API int lcu_op_attention_prefix(void *o, int stride_tok_o, int stride_head_o
                                     const lcu_kv_pages *pages, const int32_t *prefix_table, uint32_t prefix_len, const int32_t *table,
                                     int table_stride, int n_seq, const int32_t *tok_seq, const uint32_t *tok_ctx, int n, int nh, int nkvh, int dh,
                                     float scale, int dt, void *workspace, size_t workspace_len, lcu_stream_t s);
-/* probs[r, j] = exp((x_j - max) / T) / sum over the n logits of row r, f32; T = temperature[r] (device, >= 0; NULL: 1 everywhere).  T = 0: 1 at
+/* probs[r, j] = exp((x_j - max) / T) / sum over the n logits of row r, f32; T = temperature[r] (device, finite, >= 0; NULL: 1 everywhere).  T = 0: 1 at
  * the lowest index of the largest logit, 0 elsewhere.  Logits of dtype dt (F16, BF16, F32); strides from row to row in elements.
- * Logits of -inf get 0; a row of nothing else gets zeros; with T > 0 a row that holds NaN or +inf is NaN, with T = 0 NaN never is the largest. */
+ * Logits of -inf get 0; a row of nothing else gets zeros; with T > 0 a row that holds NaN or +inf is NaN, with T = 0 NaN never is the largest.
+ * probs may be the logits (F32, same stride), and may not overlap them otherwise. */
 LCU_API int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *logits, size_t stride_l, const float *temperature, int rows, size_t n, int dt,
                                 lcu_stream_t s);
 /* Verification of drafted tokens (speculative sampling) from given random numbers.  Sequence b brings n_drafted[b] <= k drafts (NULL: k

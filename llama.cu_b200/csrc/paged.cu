@@ -465,7 +465,7 @@ static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
 
 static int rows_run(RowsArgs &a, const lcu_qk_prep *prep, int n, int dt, const char *who, cudaStream_t s) {
     LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "%s: dtype %d unsupported", who, dt);
-    LCU_REQUIRE(n >= 0 && a.nh >= 0 && a.nkvh >= 0 && a.nh + a.nkvh > 0 && (long long)a.nh + 2LL * a.nkvh <= 65535, "%s: %d tokens, %d and %d heads", who, n, a.nh, a.nkvh);
+    LCU_REQUIRE(n >= 0 && n <= 0x40000000 && a.nh >= 0 && a.nkvh >= 0 && a.nh + a.nkvh > 0 && (long long)a.nh + 2LL * a.nkvh <= 65535, "%s: %d tokens, %d and %d heads", who, n, a.nh, a.nkvh);
     LCU_REQUIRE(a.dh >= 1 && a.dh <= RW_MAX_HEAD, "%s: heads of %d values (1..%d)", who, a.dh, RW_MAX_HEAD);
     const int es = dt == LCU_F32 ? 4 : 2, per = 16 / es;
     bool vec = a.dh % 8 == 0;

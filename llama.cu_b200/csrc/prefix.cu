@@ -769,8 +769,8 @@ __global__ void __launch_bounds__(256, 4) own_sum_kernel(const PrefixArgs a, int
     const int lane = threadIdx.x & 31, hkv = blockIdx.y, row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= a.plan.rows) return;
     const int seq = a.tok_seq[row / (a.nh / a.nkvh)];
+    grid_dep_wait();  // (rows of padding too: the call ends behind its kernels, which still write to the workspace)
     if (seq < 0 || seq >= a.n_seq) return;
-    grid_dep_wait();
     OwPart<PD> p;
     p.clear();
     ow_finish<T, DH>(a, p, hkv, row, splits, lane);
@@ -844,7 +844,7 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
 using namespace lcu;
 
 extern "C" size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len) {
-    if (n <= 0 || nkvh <= 0 || nh < nkvh || nh % nkvh || dh <= 0 || !prefix_len) return 0;
+    if (n <= 0 || n > 65535 || nkvh <= 0 || nkvh > 65535 || nh < nkvh || nh % nkvh || nh / nkvh > 16 || dh <= 0 || !prefix_len) return 0;  // (the call refuses these)
     return prefix_bytes(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh);
 }
 

@@ -639,7 +639,7 @@ using namespace lcu;
 extern "C" int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *logits, size_t stride_l, const float *temperature, int rows, size_t n, int dt,
                                    lcu_stream_t s) {
     LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "softmax_rows: dtype %d unsupported", dt);
-    LCU_REQUIRE(rows >= 0 && n >= 1 && n <= 0x7fffffffull && (rows <= 1 || (stride_p >= n && stride_l >= n)), "softmax_rows: %d rows of %zu, strides %zu and %zu", rows,
+    LCU_REQUIRE(rows >= 0 && rows <= 0x40000000 && n >= 1 && n <= 0x7fffffffull && (rows <= 1 || (stride_p >= n && stride_l >= n)), "softmax_rows: %d rows of %zu, strides %zu and %zu", rows,
                 n, stride_l, stride_p);
     if (rows == 0) return LCU_OK;
     LCU_REQUIRE(probs && logits, "softmax_rows: null argument");
@@ -652,7 +652,7 @@ extern "C" int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *lo
 extern "C" int lcu_op_verify_drafts(int32_t *accepted, int32_t *tokens, const void *target, size_t stride_t, const void *draft, size_t stride_d,
                                     const int32_t *drafted, const int32_t *n_drafted, const float *randoms, int n_seq, int k, size_t n, int dt, lcu_stream_t s) {
     LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16 || dt == LCU_F32, "verify_drafts: dtype %d unsupported", dt);
-    LCU_REQUIRE(n_seq >= 0 && k >= 0 && k <= 0xffff && n >= 1 && n <= 0x7fffffffull, "verify_drafts: %d sequences, %d drafts, %zu tokens", n_seq, k, n);
+    LCU_REQUIRE(n_seq >= 0 && n_seq <= 0x40000000 && k >= 0 && k <= 0xffff && n >= 1 && n <= 0x7fffffffull, "verify_drafts: %d sequences, %d drafts, %zu tokens", n_seq, k, n);
     if (n_seq == 0) return LCU_OK;
     LCU_REQUIRE(accepted && tokens && target && randoms && (k == 0 || drafted), "verify_drafts: null argument");
     LCU_REQUIRE(stride_t >= n && (!draft || k == 0 || stride_d >= n), "verify_drafts: strides %zu and %zu below %zu", stride_t, stride_d, n);

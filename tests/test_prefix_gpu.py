@@ -373,3 +373,13 @@ def test_a_speculative_round_eager_and_captured(L):
         torch.cuda.synchronize()
         check(before)
     assert math.isfinite(float(S["probs"].sum()))
+
+
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_a_call_of_padding_alone_ends_behind_its_kernels(L, tokens):
+    """What is queued behind the call finds the workspace at rest."""
+    b = Batch(77, [], 9000, 32, 8, 128, 0, 64, pad=tokens)
+    b.run(L)
+    b.ws.zero_()
+    torch.cuda.synchronize()
+    assert (b.o == 7).all() and (b.ws == 0).all()

@@ -130,3 +130,12 @@ def test_accessors_refuse(L):
     out, n = L.KvPages(), C.c_int()
     refused(L, lib.lcu_kv_layer_pages(None, 0, C.byref(out)), "null")
     refused(L, lib.lcu_seq_pages(None, 0, None, 0, C.byref(n)), "bad sequence")
+
+
+def test_counts_whose_indices_would_not_fit(L):
+    refused(L, softmax(L, rows=2 ** 30 + 1), "rows")
+    refused(L, verify(L, seqs=2 ** 30 + 1), "sequences")
+    refused(L, norm_rope(L, n=2 ** 30 + 1), "tokens")
+    refused(L, append(L, n=2 ** 30 + 1), "tokens")
+    size = L.load_library().lcu_attention_prefix_workspace_size
+    assert size(65536, 8, 2, 128, 100) == size(2 ** 31 - 1, 2 ** 31 - 1, 1, 128, 2 ** 32 - 1) == size(3, 34, 2, 128, 100) == 0  # (what the call refuses)

@@ -191,3 +191,26 @@ def test_greedy_round(L):
     assert accepted.tolist() == [3, 0, 2, 3]
     for b, a in enumerate(accepted.tolist()):
         assert tokens[b].tolist() == best[b, :a + 1].tolist() + [-1] * (k - a)
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2])
+@pytest.mark.parametrize("rows,n,pad", [(700, 2049, 0), (600, 20001, 0), (300, 50257, 6), (120, 100003, 1), (80, 200001, 0), (60, 262145, 0), (400, 5000, 3)])
+def test_softmax_of_many_rows_that_begin_inside_a_piece(L, dt, rows, n, pad):
+    """More rows than run at once, and strides that are no multiple of 16 bytes: the copy of the next row begins ahead of it."""
+    x = R.rng_normal(n + dt, (rows, n + pad), dt, 3.0)[:, :n]
+    t = torch.tensor([0.8, 1.0, 0.0, 1e-3, 50.0, 2.5, 0.3], device=DEV).repeat(rows // 7 + 1)[:rows].contiguous()
+    x[5, 3:] = -torch.inf
+    x[6] = -torch.inf
+    wide = torch.full((rows, n + pad), 7.0, device=DEV)
+    got = softmax(L, x, t, wide)[:, :n]
+    assert (wide[:, n:] == 7).all()
+    for at in range(0, rows, 100):  # (64 bits of all rows at once would take gigabytes)
+        close(got[at:at + 100], x[at:at + 100], t[at:at + 100])
+
+
+@pytest.mark.parametrize("rows,n", [(3, 1000), (1, 128256), (200, 30001), (90, 262144), (5, 300001)])
+def test_softmax_in_place(L, rows, n):
+    x = R.rng_normal(n, (rows, n), 2, 3.0)
+    t = torch.tensor([0.7, 0.0, 1.0], device=DEV).repeat(rows // 3 + 1)[:rows].contiguous()
+    want = softmax(L, x, t)
+    assert torch.equal(softmax(L, x, t, x), want)
