@@ -11,9 +11,9 @@
 //    contiguous ranges; a CTA leaves one partial result per (KV head, row tile) that it meets.
 //  - own_kernel: each token's own slots.  A CTA owns a KV head and up to 16 query rows of one sequence's consecutive tokens (drafted tokens
 //    share their keys); its two warps take 16 keys each in turns, with a softmax of their own and both products in registers (mma.sync),
-//    and meet once at the end.  It is launched as a programmatic dependent and fits on an SM beside a block of the prefix, under whose
-//    exponentials it loads.
+//    and meet once at the end.  It is launched as a programmatic dependent: its blocks run on the SMs that the prefix leaves, then on all.
 //  - The sum of all parts: at the end of own_kernel where its blocks are few, else in own_sum_kernel.
+//  - A prefix that is short next to the number of tokens is read by own_kernel too, ahead of the token's own slots, and the call is one launch.
 //
 // f32 scores and softmax, sums in f32 over the weights as they are, weights rounded to the activation type ahead of the second product (its
 // operands are 16-bit), one rounding of the output.  (Sums over the rounded weights, as attention.cu takes them, are no closer to the
@@ -31,7 +31,8 @@ struct PrefixArgs {
     lcu_kv_pages pages;
     const int32_t *prefix_table, *table, *tok_seq;
     const uint32_t *tok_ctx;
-    uint32_t prefix_len;
+    uint32_t prefix_len;  // of the parts in the workspace
+    uint32_t walk_len;    // or of what own_kernel reads itself, ahead of the token's own slots
     int table_stride, n_seq, page_shift, n, nh, nkvh;
     float scale2;  // scores in powers of two
     PrefixPlan plan;
@@ -420,11 +421,12 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
 // ------------------------------------------------------------------ own slots, and the sum
 
 constexpr int OW_KEYS = 16, OW_WARPS = 2, OW_THREADS = 32 * OW_WARPS;
-
-// A warp's keys and values: two tiles of keys, one of values.  Small enough for a block beside a block of prefix_tc_kernel, and for eight on an
-// SM of their own.
+// A warp's tiles: keys and values of the chunk that it works on and, where blocks are few, of the next (eight blocks of a ring of one on an SM, five
+// of a ring of two: 264 blocks that read 4000 slots each take 101 us with two and 122 with one, 800 blocks and 1000 slots 68 and 56).
 template <int DH> constexpr size_t ow_tile_bytes() { return (size_t)OW_KEYS * (DH + 8) * 2; }
-template <int DH> constexpr size_t ow_smem() { return (OW_WARPS * 3 + 1) * ow_tile_bytes<DH>(); }  // and the queries; later the warps' parts: 16 rows of DH f32 each
+constexpr int ow_tiles(int depth) { return OW_WARPS * 2 * depth; }
+template <int DH> constexpr size_t ow_smem(int depth) { return (ow_tiles(depth) + 1) * ow_tile_bytes<DH>(); }  // and the queries; later the warps' parts: 16 rows of DH f32 each
+static_assert(ow_smem<64>(1) >= OW_WARPS * 16 * 64 * 4 && ow_smem<128>(1) >= OW_WARPS * 16 * 128 * 4, "parts of the warps");
 template <int DH> constexpr size_t ow_part_bytes() { return (size_t)16 * DH * 4 + 16 * 8; }  // a CTA's part in the first one's memory (clusters)
 
 __device__ __forceinline__ void ow_cp16(void *dst, const void *src, bool valid) {
@@ -521,8 +523,8 @@ __device__ __forceinline__ void ow_finish(const PrefixArgs &a, OwPart<DH / 32> &
 }
 
 // grid (splits, KV heads, tokens); the splits of a token are a cluster where own_kernel adds up
-template <class T, int DH>
-__global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, int tokens_per, int splits) {
+template <class T, int DH, int DEPTH>
+__global__ void __launch_bounds__(OW_THREADS, DEPTH == 1 ? 8 : 5) own_kernel(const PrefixArgs a, int tokens_per, int splits) {
     constexpr int ROW = DH + 8, KS = DH / 16, PD = DH / 32, CH = DH / 8;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float ml[OW_WARPS][16][2];
@@ -550,78 +552,98 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
     const uint32_t lim0 = __shfl_sync(0xffffffffu, ctx, r0 / group), lim1 = __shfl_sync(0xffffffffu, ctx, r1 / group);  // 0 behind the last row
     const uint32_t lim_min = __reduce_min_sync(0xffffffffu, lane < n_tok ? ctx : 0xffffffffu);
     ctx = __reduce_max_sync(0xffffffffu, ctx);
-    const int chunks = (int)((ctx + OW_KEYS - 1) / OW_KEYS);
+    const int walked = (int)((a.walk_len + OW_KEYS - 1) / OW_KEYS), chunks = walked + (int)((ctx + OW_KEYS - 1) / OW_KEYS);  // chunks of the prefix, of all keys
 
-    T *const qs = reinterpret_cast<T *>(smem + OW_WARPS * 3 * ow_tile_bytes<DH>());  // [16][ROW], rows behind the last are zero
+    T *const qs = reinterpret_cast<T *>(smem + ow_tiles(DEPTH) * ow_tile_bytes<DH>());  // [16][ROW], rows behind the last are zero
     for (int i = tid; i < 16 * CH; i += OW_THREADS) {
         const int r = i / CH, c = 8 * (i % CH);
         const bool valid = r < rows;
         ow_cp16(qs + r * ROW + c, reinterpret_cast<const T *>(a.q) + (valid ? (size_t)(t + r / group) * a.stq + (size_t)(hkv * group + r % group) * a.shq + c : 0), valid);
     }
     ow_commit();
-    T *const k_tiles = reinterpret_cast<T *>(smem + (size_t)warp * 3 * ow_tile_bytes<DH>()), *const vs = k_tiles + 2 * OW_KEYS * ROW;
+    T *const k_tiles = reinterpret_cast<T *>(smem + (size_t)warp * 2 * DEPTH * ow_tile_bytes<DH>());  // [DEPTH] tiles of keys, then of values
     const int step = splits * OW_WARPS;
-    auto row_at = [&](int chunk) -> long long {  // lane i: where key i of the chunk lies, -1: nowhere
-        const uint32_t key = (uint32_t)chunk * OW_KEYS + (lane & 15);
-        if (chunk >= chunks || key >= ctx) return -1;
-        const int page = a.table[(size_t)seq * a.table_stride + (key >> a.page_shift)];
-        if (page < 0 || page >= a.pages.n_pages) return -1;
-        return (long long)page * a.pages.stride_page + (long long)(key & ((1u << a.page_shift) - 1)) * a.pages.stride_tok + (long long)hkv * a.pages.stride_head;
+    // lane i: key i of a chunk.  The id of its page is loaded a step ahead of its use.
+    auto page_of = [&](int chunk) {
+        const bool shared = chunk < walked;
+        const uint32_t key = (uint32_t)(shared ? chunk : chunk - walked) * OW_KEYS + (lane & 15);
+        if (chunk >= chunks || key >= (shared ? a.walk_len : ctx)) return -1;
+        return shared ? a.prefix_table[key >> a.page_shift] : a.table[(size_t)seq * a.table_stride + (key >> a.page_shift)];
     };
-    auto request = [&](T *dst, const void *base, long long at) {
+    auto request = [&](int chunk, int page, int tile) {  // its keys and values, zeros where there are none; which there are
+        const uint32_t key = (uint32_t)(chunk < walked ? chunk : chunk - walked) * OW_KEYS + (lane & 15);
+        const bool valid = page >= 0 && page < a.pages.n_pages;
+        const long long at = valid ? (long long)page * a.pages.stride_page + (long long)(key & ((1u << a.page_shift) - 1)) * a.pages.stride_tok + (long long)hkv * a.pages.stride_head : 0;
+        const unsigned some = __ballot_sync(0xffffffffu, valid);
+        if (chunk < chunks) {
+            T *const kd = k_tiles + tile * OW_KEYS * ROW + lane / CH * ROW + 8 * (lane % CH), *const vd = kd + DEPTH * OW_KEYS * ROW;
 #pragma unroll
-        for (int i = 0; i < OW_KEYS * CH / 32; ++i) {
-            const int key = lane / CH + i * (32 / CH), c = 8 * (lane % CH);
-            const long long off = __shfl_sync(0xffffffffu, at, key);
-            ow_cp16(dst + key * ROW + c, reinterpret_cast<const T *>(base) + (off < 0 ? 0 : off + c), off >= 0);
+            for (int i = 0; i < OW_KEYS * CH / 32; ++i) {
+                const int k = lane / CH + i * (32 / CH);
+                const long long off = __shfl_sync(0xffffffffu, at, k) + 8 * (lane % CH);
+                const bool is = some >> k & 1u;
+                ow_cp16(kd + i * (32 / CH) * ROW, reinterpret_cast<const T *>(a.pages.k) + off, is);
+                ow_cp16(vd + i * (32 / CH) * ROW, reinterpret_cast<const T *>(a.pages.v) + off, is);
+            }
         }
+        ow_commit();
+        return some & 0xffffu;
     };
     float o[DH / 8][4];
 #pragma unroll
     for (int i = 0; i < DH / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    // Copies in flight, in this order: keys of this chunk, its values, keys of the next; page ids of the one behind.
+    // Keys and values of DEPTH chunks in flight, and the page ids of the one behind them.
     const int c0 = split * OW_WARPS + warp;
-    long long at0 = row_at(c0), at1 = row_at(c0 + step), at2 = row_at(c0 + 2 * step);
-    if (c0 < chunks) {
-        request(k_tiles, a.pages.k, at0);
-        ow_commit();
-        request(vs, a.pages.v, at0);
-        ow_commit();
-        request(k_tiles + OW_KEYS * ROW, a.pages.k, at1);
-        ow_commit();
+    unsigned there[DEPTH];  // which keys of each there are
+    {
+        int page[DEPTH];
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) page[i] = page_of(c0 + i * step);
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) there[i] = request(c0 + i * step, page[i], i);
     }
-    if (c0 < chunks) ow_wait<3>();
-    else ow_wait<0>();
+    int page_next = page_of(c0 + DEPTH * step);
+    ow_wait<DEPTH>();
     __syncthreads();  // the queries are there
     int tile = 0;
     for (int c = c0; c < chunks; c += step) {
-        const unsigned there = __ballot_sync(0xffffffffu, at0 >= 0);
-        const T *ks = k_tiles + tile * OW_KEYS * ROW;
-        ow_wait<2>();
-        float s[2][4] = {};
+        const unsigned here = there[0];
+        T *const ks = k_tiles + tile * OW_KEYS * ROW, *const vs = ks + DEPTH * OW_KEYS * ROW;
+        ow_wait<DEPTH - 1>();
+        const uint32_t first = (uint32_t)(c < walked ? 0 : c - walked) * OW_KEYS;  // of the token's own slots
+        const uint32_t see0 = c < walked ? 0xffffffffu : lim0, see1 = c < walked ? 0xffffffffu : lim1;
+        float s[2][4] = {}, s2[2][4] = {};  // two chains of products each
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+        for (int k = 0; k < KS; k += 2) {
             uint32_t qa[4], b[4];
             ow_ldm4(qa, qs + (lane & 15) * ROW + 16 * k + (lane >> 4) * 8);
             ow_ldm4(b, ks + ((lane & 7) + (lane >> 4) * 8) * ROW + 16 * k + (lane >> 3 & 1) * 8);
             mma16816<T>(s[0], qa[0], qa[1], qa[2], qa[3], b[0], b[1]);
             mma16816<T>(s[1], qa[0], qa[1], qa[2], qa[3], b[2], b[3]);
+            ow_ldm4(qa, qs + (lane & 15) * ROW + 16 * k + 16 + (lane >> 4) * 8);
+            ow_ldm4(b, ks + ((lane & 7) + (lane >> 4) * 8) * ROW + 16 * k + 16 + (lane >> 3 & 1) * 8);
+            mma16816<T>(s2[0], qa[0], qa[1], qa[2], qa[3], b[0], b[1]);
+            mma16816<T>(s2[1], qa[0], qa[1], qa[2], qa[3], b[2], b[3]);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[h][e] += s2[h][e];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int i = 8 * h + 2 * t4 + e;
-                const uint32_t key = (uint32_t)c * OW_KEYS + i;
-                const bool seen = there >> i & 1u;
-                s[h][e] = seen && key < lim0 ? s[h][e] * a.scale2 : -INFINITY;
-                s[h][2 + e] = seen && key < lim1 ? s[h][2 + e] * a.scale2 : -INFINITY;
+                const uint32_t key = first + i;
+                const bool seen = here >> i & 1u;
+                s[h][e] = seen && key < see0 ? s[h][e] * a.scale2 : -INFINITY;
+                s[h][2 + e] = seen && key < see1 ? s[h][2 + e] * a.scale2 : -INFINITY;
             }
         const float n0 = fmaxf(m0, ow_quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]))));
         const float n1 = fmaxf(m1, ow_quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]))));
         const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-        const float f0 = m0 == -INFINITY ? 0.f : at_exp2(m0 - b0), f1 = m1 == -INFINITY ? 0.f : at_exp2(m1 - b1);
+        const float f0 = m0 == -INFINITY ? 1.f : at_exp2(m0 - b0), f1 = m1 == -INFINITY ? 1.f : at_exp2(m1 - b1);  // (a row that has seen nothing has nothing to scale)
         m0 = n0;
         m1 = n1;
         uint32_t pa[4];
@@ -642,10 +664,9 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
                 o[i][3] *= f1;
             }
         }
-        ow_wait<1>();
         // Keys that one token of the group sees and another does not: a weight of zero times a value that is not finite would be NaN.
         bool odd = false;
-        if ((uint32_t)(c + 1) * OW_KEYS > lim_min && lim_min < ctx)
+        if (c >= walked && first + OW_KEYS > lim_min && lim_min < ctx)
             for (int i = lane; i < OW_KEYS * DH / 2; i += 32) {
                 const float2 v = Act<T>::to_f2(*reinterpret_cast<const uint32_t *>(vs + i / (DH / 2) * ROW + i % (DH / 2) * 2));
                 odd = odd || !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY);
@@ -656,8 +677,8 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
                 const int from = (lane & ~3) | (i & 7) >> 1;  // the lane that has the weights of key i
                 const float2 u0 = Act<T>::to_f2(__shfl_sync(0xffffffffu, i < 8 ? pa[0] : pa[2], from)), u1 = Act<T>::to_f2(__shfl_sync(0xffffffffu, i < 8 ? pa[1] : pa[3], from));
                 const float x0 = i & 1 ? u0.y : u0.x, x1 = i & 1 ? u1.y : u1.x;
-                const uint32_t key = (uint32_t)c * OW_KEYS + i;
-                const bool seen = there >> i & 1u;
+                const uint32_t key = first + i;
+                const bool seen = here >> i & 1u;
 #pragma unroll
                 for (int d = 0; d < DH / 8; ++d) {
                     const float2 v = Act<T>::to_f2(*reinterpret_cast<const uint32_t *>(vs + i * ROW + 8 * d + 2 * t4));
@@ -679,15 +700,12 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
             mma16816<T>(o[2 * i], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
             mma16816<T>(o[2 * i + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
         }
-        __syncwarp();  // values and this tile of keys may be replaced
-        request(vs, a.pages.v, at1);
-        ow_commit();
-        request(k_tiles + tile * OW_KEYS * ROW, a.pages.k, at2);
-        ow_commit();
-        at0 = at1;
-        at1 = at2;
-        at2 = row_at(c + 3 * step);
-        tile ^= 1;
+        __syncwarp();  // this tile of keys and of values may be replaced
+#pragma unroll
+        for (int i = 0; i + 1 < DEPTH; ++i) there[i] = there[i + 1];
+        there[DEPTH - 1] = request(c + DEPTH * step, page_next, tile);
+        page_next = page_of(c + (DEPTH + 1) * step);
+        if (++tile == DEPTH) tile = 0;
     }
     ow_wait<0>();
     l0 = ow_quad_sum(l0);
@@ -716,7 +734,7 @@ __global__ void __launch_bounds__(OW_THREADS, 8) own_kernel(const PrefixArgs a, 
         return p;
     };
     if (cluster) {
-        float *const cluster_o = reinterpret_cast<float *>(smem + ow_smem<DH>());  // in the first CTA: [split][16][DH], then (m, l) [split][16]
+        float *const cluster_o = reinterpret_cast<float *>(smem + ow_smem<DH>(DEPTH));  // in the first CTA: [split][16][DH], then (m, l) [split][16]
         float *const cluster_ml = cluster_o + (size_t)splits * 16 * DH;
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 #pragma unroll 1
@@ -790,38 +808,22 @@ static int pf_map(CUtensorMap *m, int dt, const void *base, const lcu_kv_pages &
     return LCU_OK;
 }
 
-template <class T, int DH>
-static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
+template <class T, int DH, int DEPTH>
+static int own_run(const PrefixArgs &a, int splits, bool cluster, cudaStream_t s) {
     static OncePerDevice once;
     const int set = once.run([]() -> int {
-        LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem<DH>()));
-        LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>() + 8 * ow_part_bytes<DH>())));
+        LCU_CHECK_CUDA(cudaFuncSetAttribute(own_kernel<T, DH, DEPTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ow_smem<DH>(DEPTH) + 8 * ow_part_bytes<DH>())));
         return LCU_OK;
     });
     if (set) return set;
-    if (a.prefix_len) {
-        CUtensorMap mk, mv;
-        int rc = pf_map(&mk, dt, a.pages.k, a.pages, DH, a.nkvh);
-        if (!rc) rc = pf_map(&mv, dt, a.pages.v, a.pages, DH, a.nkvh);
-        if (rc) return rc;
-        LCU_CHECK_CUDA(launch_kernel(prefix_tc_kernel<T, DH>, dim3(a.plan.ctas), dim3(PF_THREADS), pf_smem<DH>(), s, false, a, mk, mv, dt == LCU_BF16 ? 1u : 0u));
-    }
-    const int group = a.nh / a.nkvh, tokens_per = 16 / group;
-    // keys of long contexts: over a cluster where blocks are few, over blocks that leave a part each where there are more
-    const long long cap = (long long)a.table_stride << a.page_shift, blocks = (long long)a.nkvh * a.n;
-    const bool leave = a.prefix_len && a.plan.own_parts;
-    int splits = 1;
-    if (leave) splits = (int)(cap < 64LL * a.plan.own_parts ? (cap + 63) / 64 > 0 ? (cap + 63) / 64 : 1 : a.plan.own_parts);
-    else while (splits < 8 && blocks * splits <= sm_count() && cap > (long long)splits * 64) splits *= 2;
-    const size_t smem = ow_smem<DH>() + (splits > 1 && !leave ? splits * ow_part_bytes<DH>() : 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.nkvh, a.n);
     cfg.blockDim = dim3(OW_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = ow_smem<DH>(DEPTH) + (cluster ? splits * ow_part_bytes<DH>() : 0);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
-    if (splits > 1 && !leave) {
+    if (cluster) {
         attr[n_attr].id = cudaLaunchAttributeClusterDimension;
         attr[n_attr].val.clusterDim.x = splits;
         attr[n_attr].val.clusterDim.y = attr[n_attr].val.clusterDim.z = 1;
@@ -834,7 +836,34 @@ static int prefix_run(PrefixArgs &a, int dt, cudaStream_t s) {
     }
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
-    LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, own_kernel<T, DH>, (const PrefixArgs)a, tokens_per, splits));
+    LCU_CHECK_CUDA(cudaLaunchKernelEx(&cfg, own_kernel<T, DH, DEPTH>, a, 16 / (a.nh / a.nkvh), splits));
+    return LCU_OK;
+}
+
+template <class T, int DH>
+static int prefix_run(const PrefixArgs &a, int dt, cudaStream_t s) {
+    if (a.prefix_len) {
+        static OncePerDevice once;
+        const int set = once.run([]() -> int {
+            LCU_CHECK_CUDA(cudaFuncSetAttribute(prefix_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_smem<DH>()));
+            return LCU_OK;
+        });
+        if (set) return set;
+        CUtensorMap mk, mv;
+        int rc = pf_map(&mk, dt, a.pages.k, a.pages, DH, a.nkvh);
+        if (!rc) rc = pf_map(&mv, dt, a.pages.v, a.pages, DH, a.nkvh);
+        if (rc) return rc;
+        LCU_CHECK_CUDA(launch_kernel(prefix_tc_kernel<T, DH>, dim3(a.plan.ctas), dim3(PF_THREADS), pf_smem<DH>(), s, false, a, mk, mv, dt == LCU_BF16 ? 1u : 0u));
+    }
+    // keys of long contexts: over a cluster where blocks are few, over blocks that leave a part each where there are more
+    const long long cap = a.walk_len + ((long long)a.table_stride << a.page_shift), blocks = (long long)a.nkvh * a.n;
+    const bool leave = a.prefix_len && a.plan.own_parts;
+    int splits;
+    if (leave) splits = (int)(cap < 64LL * a.plan.own_parts ? (cap + 63) / 64 > 0 ? (cap + 63) / 64 : 1 : a.plan.own_parts);
+    else splits = own_splits(blocks, cap, sm_count());
+    const bool cluster = splits > 1 && !leave;
+    const int rc = blocks * splits <= 5LL * sm_count() ? own_run<T, DH, 2>(a, splits, cluster, s) : own_run<T, DH, 1>(a, splits, cluster, s);
+    if (rc) return rc;
     if (leave) LCU_CHECK_CUDA(launch_kernel(own_sum_kernel<T, DH>, dim3((a.plan.rows + 7) / 8, a.nkvh), dim3(256), 0, s, true, a, splits));
     return LCU_OK;
 }
@@ -875,7 +904,10 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.tok_ctx = tok_ctx;
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
     a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale * 1.4426950408889634f;
-    if (prefix_len) {
+    if (prefix_len && prefix_walk(n, nh / nkvh, nkvh, prefix_len, (long long)table_stride * pages->page_tokens, sm_count(), dh)) {
+        a.walk_len = prefix_len;
+        a.prefix_len = 0;
+    } else if (prefix_len) {
         a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh, (long long)(n_seq < n ? n_seq : n) * table_stride * pages->page_tokens);
         a.part_ml = reinterpret_cast<float2 *>(workspace);
         a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan, nkvh));

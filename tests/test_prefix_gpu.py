@@ -383,3 +383,55 @@ def test_a_call_of_padding_alone_ends_behind_its_kernels(L, tokens):
     b.ws.zero_()
     torch.cuda.synchronize()
     assert (b.o == 7).all() and (b.ws == 0).all()
+
+
+# Behind thousands of tokens (padding but for a few) the prefix is on the tensor cores however short it is; behind a few, the blocks of the own slots read it.
+@pytest.mark.parametrize("dt,dh", [(0, 128), (1, 64)])
+@pytest.mark.parametrize("prefix,pad", [(8, 30000), (9, 30000), (63, 1500), (64, 1500), (65, 1500), (127, 1000), (129, 1000), (255, 500), (257, 500)])
+def test_short_prefixes_of_many_tokens(L, dt, dh, prefix, pad):
+    b = Batch(prefix + dh, [(3, 1), (40, 2), (0 + 1, 1)], prefix, 32, 8, dh, dt, 16, pad=pad, std=2.0)
+    few = Batch(prefix + dh, [(3, 1), (40, 2), (0 + 1, 1)], prefix, 32, 8, dh, dt, 16, pad=2, std=2.0)
+    few.q, few.pool, few.prefix_ids, few.ids = b.q[:few.n].clone(), b.pool, b.prefix_ids, b.ids
+    b.run(L)
+    few.run(L)
+    few.check()
+    assert (b.o[4:] == 7).all()
+    b.n, b.tok_seq, b.ctx = 4, b.tok_seq[:4], b.ctx[:4]
+    b.check()
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 128])
+@pytest.mark.parametrize("pad", [0, 900])
+def test_prefix_pages_that_name_no_page(L, page, pad):
+    """Few tokens and many: the slots of such pages are not seen, whoever reads the prefix."""
+    b = Batch(page, [(20, 1), (page + 3, 3)], 300, 32, 8, 128, 1, page, pad=pad)
+    b.prefix_ids[1], b.prefix_ids[-1] = -1, b.n_pages
+    if len(b.prefix_ids) > 4:
+        b.prefix_ids[3] = 2 ** 31 - 1
+    b.ids[1, 0] = -7
+    b.run(L)
+    b.n, b.tok_seq, b.ctx = 4, b.tok_seq[:4], b.ctx[:4]
+    b.check()
+
+
+@pytest.mark.parametrize("pad", [0, 900])
+@pytest.mark.parametrize("filth", [math.nan, math.inf])
+def test_filth_behind_a_prefix_and_behind_contexts(L, pad, filth):
+    """Slots that nobody sees: of the prefix's last page, of the sequences', of pages of others."""
+    b = Batch(31, [(5, 1), (37, 3), (1, 1)], 201, 32, 8, 128, 0, 32, pad=pad)
+    keep = torch.zeros(b.pool.shape[0], 32, dtype=torch.bool)
+    for ids, count in [(b.prefix_ids, 201), (b.ids[0], 5), (b.ids[1], 37), (b.ids[2], 1)]:
+        for s in range(count):
+            keep[ids[s // 32], s % 32] = True
+    b.pool.masked_fill_(~keep.to(DEV)[:, None, None, :, None], filth)
+    b.run(L)
+    b.n, b.tok_seq, b.ctx = 5, b.tok_seq[:5], b.ctx[:5]
+    b.check()
+
+
+@pytest.mark.parametrize("dh,nh,nkvh", [(128, 32, 32), (64, 24, 8), (128, 64, 4), (64, 5, 5)])
+@pytest.mark.parametrize("tokens,own", [(1, 3000), (20, 700), (300, 90)])
+def test_own_contexts_of_few_and_many_blocks(L, dh, nh, nkvh, tokens, own):
+    b = Batch(dh + tokens, [(1 + (own * (i + 1)) // tokens, 1) for i in range(tokens)], 0 if tokens > 20 else 70, nh, nkvh, dh, 1, 16)
+    b.run(L)
+    b.check()

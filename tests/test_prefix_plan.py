@@ -22,7 +22,7 @@ int main() {
                lcu::prefix_ml_bytes(p, nkvh) + lcu::prefix_part_rows(p, nkvh) * dh * 4, lcu::prefix_bytes(n, group, nkvh, len, sms, dh));
         const long long show = p.pairs < 5000 ? p.pairs : 5000;
         for (long long i = 0; i < show; ++i) printf(" %lld %lld", p.first_cta(i), p.last_cta(i));
-        printf("\n");
+        printf(" %d %d\n", lcu::prefix_walk(n, group, nkvh, len, own, sms, dh), lcu::own_splits((long long)n * nkvh, own + len, sms));
     }
 }
 """
@@ -48,7 +48,7 @@ def test_every_unit_belongs_to_one_cta_and_every_piece_has_a_slot(plans):
     for shape, p in zip(SHAPES, plans(SHAPES)):
         n, group, nkvh, length, _, _ = shape
         pairs, units, per, ctas, key_tiles, slot_rows, parts, own_row, used, bound = p[:10]
-        ends = list(zip(p[10::2], p[11::2]))
+        ends = list(zip(p[10:-2:2], p[11:-2:2]))
         assert key_tiles == -(-length // 128) and pairs == nkvh * -(-n * group // 256) and units == pairs * key_tiles, shape
         assert 1 <= ctas <= SMS and (ctas - 1) * per < units <= ctas * per, shape  # every CTA has units: none meets a range that is empty
         slots = set()
@@ -65,7 +65,7 @@ def test_every_unit_belongs_to_one_cta_and_every_piece_has_a_slot(plans):
 def test_parts_of_own_slots(plans):
     for shape, p in zip(SHAPES, plans(SHAPES)):
         blocks, parts = shape[0] * shape[2], p[6]
-        assert parts == 0 if blocks <= SMS else 1 <= parts <= 12 and (parts == 1 or parts * blocks <= 12 * SMS), shape
+        assert parts == 0 if blocks <= SMS else 1 <= parts <= 3 and (parts == 1 or parts * blocks <= 3 * SMS), shape
 
 
 def test_the_largest_call(plans):
@@ -105,3 +105,21 @@ def test_a_softmax_whose_wait_ran_out_is_nan_and_leaves_after_its_copy():
     body = text[text.index("softmax_kernel(const SoftmaxArgs"):text.index("struct VerifyArgs")]
     assert "if (AHEAD && !here) keep[0] = nan" in body and re.search(r"if \(!exchange\(.*\)\) s = nan", body) and "!here ? nan" in body
     assert body.rstrip().endswith("}") and "if (abort_flag) tc_warp_drain(tc_smem(&bar)" in body
+
+
+def test_a_prefix_is_read_by_the_blocks_of_the_own_slots_while_that_is_short(plans):
+    def walks(n, length, group=4, nkvh=8, dh=128, own=100):
+        return plans([(n, group, nkvh, length, dh, own)])[0][-2]
+    for n, short, long in ((1, 2000, 4000), (8, 1000, 2000), (33, 300, 1000), (100, 100, 300)):  # both measured
+        assert walks(n, short) and not walks(n, long), n
+    for n in (1, 3, 8, 33, 100, 1000, 20000):  # once too long, always
+        kinds = [walks(n, length) for length in (1, 8, 16, 100, 500, 1000, 2000, 4000, 8000, 32000, 2 ** 31 - 1)]
+        assert kinds == sorted(kinds, reverse=True) and kinds[0] and not kinds[-1], n
+    for n, length in ((30000, 8), (1500, 63), (1000, 127), (500, 255)):  # what the GPU's tests of short prefixes rely on
+        assert not walks(n, length) and not walks(n, length, dh=64) and walks(6, length) and walks(6, length, dh=64)
+
+
+def test_splits_of_own_slots(plans):
+    for shape, p in zip(SHAPES, plans(SHAPES)):
+        blocks, slots, splits = shape[0] * shape[2], shape[5] + shape[3], p[-1]
+        assert splits in (1, 2, 4, 8) and (splits == 1 or (blocks * splits // 2 <= SMS and slots > 64 * (splits // 2))), shape
