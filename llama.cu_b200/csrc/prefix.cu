@@ -7,8 +7,8 @@
 //
 //  - prefix_tc_kernel: the prefix, for all tokens at once, on the 5th-generation tensor cores.  The query rows (token, head of the group) of
 //    a KV head fill tiles of 256 rows, so the prefix is read once per 256 rows instead of once per token; the roles, tensor memory and
-//    arithmetic are those of attention_tc.cu.  The units (KV head, row tile, key tile) are dealt to one CTA per SM in equal
-//    contiguous ranges; a CTA leaves one partial result per (KV head, row tile) that it meets.
+//    arithmetic are those of attention_tc.cu.  The units (KV head, row tile, key tile) are dealt to one CTA per SM in
+//    contiguous ranges of equal cost; a CTA leaves one partial result per (KV head, row tile) that it meets.
 //  - own_kernel: each token's own slots.  A CTA owns a KV head and up to 16 query rows of one sequence's consecutive tokens (drafted tokens
 //    share their keys); its two warps take 16 keys each in turns, with a softmax of their own and both products in registers (mma.sync),
 //    and meet once at the end.  It is launched as a programmatic dependent: its blocks run on the SMs that the prefix leaves, then on all.
@@ -49,6 +49,7 @@ constexpr int PF_MAX_STAGES = 4;
 struct PfShared {
     unsigned long long k_full[PF_MAX_STAGES], k_empty[PF_MAX_STAGES], v_full[PF_MAX_STAGES], v_empty[PF_MAX_STAGES];
     unsigned long long q_full[2], s_full[2], p_ready[2][2], pv_done[2], drain;
+    volatile int unit0, unit1;  // of the CTA (read where they are needed: registers are short)
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -85,25 +86,23 @@ __device__ __forceinline__ void pf_st32(float *p, const uint32_t *r) {  // 32 by
 
 // what a CTA does of one (KV head, row tile)
 struct PfPiece {
-    long long unit, end, pair;  // first unit, first unit behind the CTA's range
+    int unit, pair;  // first unit
     int hkv, row0, rows, j0, j1;
     bool two;
 };
-__device__ __forceinline__ PfPiece pf_piece(const PrefixPlan &pl, long long unit, long long end) {
+__device__ __forceinline__ PfPiece pf_piece(const PrefixPlan &pl, int unit, int end) {  // end: first unit behind the CTA's range
     PfPiece p;
     p.unit = unit;
-    p.end = end;
     p.pair = unit / pl.key_tiles;
-    p.j0 = (int)(unit - p.pair * pl.key_tiles);
-    const long long left = end - unit;
-    p.j1 = left < pl.key_tiles - p.j0 ? p.j0 + (int)left : pl.key_tiles;
-    p.hkv = (int)(p.pair / pl.row_tiles);
-    p.row0 = (int)(p.pair - (long long)p.hkv * pl.row_tiles) * PF_ROWS;
+    p.j0 = unit - p.pair * pl.key_tiles;
+    p.j1 = min(pl.key_tiles, p.j0 + (end - unit));
+    p.hkv = p.pair / pl.row_tiles;
+    p.row0 = (p.pair - p.hkv * pl.row_tiles) * PF_ROWS;
     p.rows = min(PF_ROWS, pl.rows - p.row0);
     p.two = p.rows > 128;
     return p;
 }
-__device__ __forceinline__ PfPiece pf_next(const PrefixPlan &pl, const PfPiece &p) { return pf_piece(pl, p.unit + (p.j1 - p.j0), p.end); }
+__device__ __forceinline__ PfPiece pf_next(const PrefixPlan &pl, const PfPiece &p, int end) { return pf_piece(pl, p.unit + (p.j1 - p.j0), end); }
 
 template <class T, int DH>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -115,7 +114,6 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
     PfShared *sh = reinterpret_cast<PfShared *>(Vs + ST * TILE);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     grid_dep_launch();
-    const long long u0 = (long long)blockIdx.x * a.plan.per, u1 = u0 + a.plan.per < a.plan.units ? u0 + a.plan.per : a.plan.units;
     const int ppt = 128 >> a.page_shift, n_prefix_pages = (int)((a.prefix_len + a.pages.page_tokens - 1) >> a.page_shift);  // pages of a tile, of all
 
     if (tid == 0) {
@@ -134,6 +132,8 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
             tc_mbar_init(tc_smem(&sh->pv_done[t]), 1);
         }
         sh->abort_flag = 0;
+        sh->unit0 = a.plan.unit_at(blockIdx.x * (unsigned)a.plan.per);
+        sh->unit1 = a.plan.unit_at((blockIdx.x + 1) * (unsigned)a.plan.per);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -150,13 +150,14 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         // ---------------- TMA producer: the ring runs on through all pieces
         const uint32_t kf = tc_smem(&sh->k_full[0]), ke = tc_smem(&sh->k_empty[0]), vf = tc_smem(&sh->v_full[0]), ve = tc_smem(&sh->v_empty[0]);
         const int pt = a.pages.page_tokens;
+        const int u0 = sh->unit0, u1 = sh->unit1;
         auto page_of = [&](int tile) {  // lane i: page i of the tile; an id that names no page is one behind the map, which reads zeros
             const int i = tile * ppt + lane;
             const int id = lane < ppt && i < n_prefix_pages ? a.prefix_table[i] : 0;
             return id < 0 || id >= a.pages.n_pages ? a.pages.n_pages : id;
         };
-        int slot = 0, hkv = (int)(u0 / a.plan.key_tiles / a.plan.row_tiles), j = (int)(u0 % a.plan.key_tiles);
-        long long pair = u0 / a.plan.key_tiles;
+        int slot = 0, hkv = u0 / a.plan.key_tiles / a.plan.row_tiles, j = u0 % a.plan.key_tiles;
+        int pair = u0 / a.plan.key_tiles;
         int id = page_of(j);
         auto load = [&](uint32_t dst, const CUtensorMap *map, uint32_t bar, int n) {
             tc_warp_expect_tx(bar, (uint32_t)(n * pt * 128 * NB));
@@ -167,7 +168,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         };
         uint32_t phase = 1;
         bool ok = true;
-        for (long long u = u0; u < u1; ++u) {
+        for (int u = u0; u < u1; ++u) {
             const int n = min(ppt, n_prefix_pages - j * ppt);
             ok = tc_warp_wait(ke + 8 * slot, phase, &sh->abort_flag);
             if (!ok) break;
@@ -180,7 +181,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
             if (++j == a.plan.key_tiles) {
                 j = 0;
                 ++pair;
-                hkv = (int)(pair / a.plan.row_tiles);
+                hkv = pair / a.plan.row_tiles;
             }
             if (u + 1 < u1) id = page_of(j);
             if (++slot == ST) { slot = 0; phase ^= 1u; }
@@ -202,7 +203,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         int slot = 0;
         uint32_t phase = 0, p_phase = 0, q_phase = 0, seen = 0;  // bit t of the last three: tile t's; whether it has had products
         bool ok = true;
-        for (PfPiece p = pf_piece(a.plan, u0, u1); ok && p.unit < u1; p = pf_next(a.plan, p)) {
+        for (PfPiece p = pf_piece(a.plan, sh->unit0, sh->unit1); ok && p.unit < sh->unit1; p = pf_next(a.plan, p, sh->unit1)) {
             const int nt = p.two ? 2 : 1;
             for (int t = 0; t < nt && ok; ++t) {
                 ok = tc_warp_wait(qf + 8 * t, q_phase >> t & 1u, &sh->abort_flag);
@@ -283,9 +284,9 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         int it = 0;          // units of the CTA so far
         uint32_t mine = 0;   // ... that had this tile
         bool ok = true;
-        PfPiece p = pf_piece(a.plan, u0, u1);
+        PfPiece p = pf_piece(a.plan, sh->unit0, sh->unit1);
         if (t == 0 || p.two) load_q(p);
-        while (p.unit < u1) {
+        while (p.unit < sh->unit1) {
             const bool active = t == 0 || p.two, some = active && 128 * t + q * 32 < p.rows;  // ... of this warp's rows
             float ref = -INFINITY, l = 0.f;
             if (active) {
@@ -371,9 +372,9 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                 if (!ok) break;
             }
             it += p.j1 - p.j0;
-            const PfPiece next = pf_next(a.plan, p);
+            const PfPiece next = pf_next(a.plan, p, sh->unit1);
             // the products of this tile's scores have ended (their last commit was waited for): its queries may be replaced
-            if (next.unit < u1 && (t == 0 || next.two)) load_q(next);
+            if (next.unit < sh->unit1 && (t == 0 || next.two)) load_q(next);
             if (active) {
                 ok = tc_mbar_wait(tc_smem(&sh->pv_done[t]), (mine - 1) & 1u, &sh->abort_flag);  // (those before it had ended when the last scores were issued)
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -408,7 +409,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
             tc_warp_commit(tc_smem(&sh->drain));
             tc_warp_drain(tc_smem(&sh->drain), 0u);
         }
-        for (PfPiece p = pf_piece(a.plan, u0, u1); p.unit < u1; p = pf_next(a.plan, p))
+        for (PfPiece p = pf_piece(a.plan, sh->unit0, sh->unit1); p.unit < sh->unit1; p = pf_next(a.plan, p, sh->unit1))
             for (int r = tid; r < p.rows; r += PF_THREADS) a.part_ml[(size_t)(blockIdx.x + p.pair) * a.plan.slot_rows + r] = make_float2(0.f, __int_as_float(0x7fc00000));
         __syncthreads();
     }
@@ -481,8 +482,8 @@ __device__ __forceinline__ void ow_finish(const PrefixArgs &a, OwPart<DH / 32> &
     constexpr int PD = DH / 32, AHEAD = 8;
     const int group = a.nh / a.nkvh, tok = row / group;
     if (a.prefix_len) {
-        const long long pair = (long long)hkv * a.plan.row_tiles + row / PF_ROWS, first = a.plan.first_cta(pair);
-        const int shared = (int)(a.plan.last_cta(pair) - first) + 1, parts = shared + own;
+        const int pair = hkv * a.plan.row_tiles + row / PF_ROWS, first = a.plan.first_cta(pair);
+        const int shared = a.plan.last_cta(pair) - first + 1, parts = shared + own;
         const size_t at0 = (size_t)(first + pair) * a.plan.slot_rows + row % PF_ROWS, at1 = a.own_row + (size_t)hkv * a.plan.rows + row;
         const size_t apart1 = (size_t)a.nkvh * a.plan.rows;
         auto at = [&](int s) { return s < shared ? at0 + (size_t)s * a.plan.slot_rows : at1 + (size_t)(s - shared) * apart1; };
@@ -873,7 +874,7 @@ static int prefix_run(const PrefixArgs &a, int dt, cudaStream_t s) {
 using namespace lcu;
 
 extern "C" size_t lcu_attention_prefix_workspace_size(int n, int nh, int nkvh, int dh, uint32_t prefix_len) {
-    if (n <= 0 || n > 65535 || nkvh <= 0 || nkvh > 65535 || nh < nkvh || nh % nkvh || nh / nkvh > 16 || dh <= 0 || !prefix_len) return 0;  // (the call refuses these)
+    if (n <= 0 || n > 65535 || nkvh <= 0 || nkvh > 65535 || nh < nkvh || nh % nkvh || nh / nkvh > 16 || dh <= 0 || !prefix_len || !prefix_fits(n, nh / nkvh, nkvh, prefix_len)) return 0;  // (the call refuses these)
     return prefix_bytes(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh);
 }
 
@@ -891,6 +892,7 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     LCU_REQUIRE(prefix_len <= 0x7fffffffu && table_stride >= 0 && (long long)table_stride * pages->page_tokens <= 0x7fffffffll && n_seq >= 1,
                 "attention_prefix: prefix of %u, %d sequences of %d pages", prefix_len, n_seq, table_stride);
     if (n == 0) return LCU_OK;
+    LCU_REQUIRE(!prefix_len || prefix_fits(n, nh / nkvh, nkvh, prefix_len), "attention_prefix: prefix of %u for %d tokens of %d heads: more than a call takes", prefix_len, n, nh);
     LCU_REQUIRE(o && q && tok_seq && tok_ctx && (prefix_table || !prefix_len) && (table || !table_stride), "attention_prefix: null argument");
     LCU_REQUIRE((((uintptr_t)o | (uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v) % 16) == 0 && (sto | sho | stq | shq) % 8 == 0 &&
                     pages->stride_page % 8 == 0 && pages->stride_tok % 8 == 0 && pages->stride_head % 8 == 0 && pages->stride_head > 0,

@@ -13,22 +13,35 @@ namespace lcu {
 
 constexpr int PF_ROWS = 256, PF_TILE = 128;  // query rows of a row tile (two MMA tiles), positions of a key tile
 
-// The units (KV head, row tile, key tile) in this order are dealt to the CTAs in equal contiguous ranges; what a CTA does of one
-// (KV head, row tile) is a piece with a partial result of its own.  CTA c's piece of pair p has number c + p: both only grow along the
+// The units (KV head, row tile, key tile) in this order are dealt to the CTAs in contiguous ranges of equal cost; what a CTA does of one
+// (KV head, row tile) is a piece with a partial result of its own.  A unit costs 1, or, where a KV head's last row tile fills one MMA tile
+// and the others two, 2 there and 3 elsewhere (measured: 1.7 and 2.4 us).  CTA c's piece of pair p has number c + p: both only grow along the
 // units, and each piece begins a new CTA or a new pair, so no two pieces share a number.
 struct PrefixPlan {
     int rows;        // query rows of a KV head: tokens x heads of its group
     int row_tiles, key_tiles;
-    long long pairs, units, per;  // (KV head, row tile); all units; units of a CTA
-    int ctas;
+    int pairs, units, per;        // (KV head, row tile); all units; cost of a CTA
+    int ctas, cost, cost_last;    // of a unit; of one in a KV head's last row tile
     int slot_rows;   // rows of a piece's slot
     // More (KV head, token) blocks for the own slots than SMs: they leave their parts too, at most so many of a row, and a kernel of its
     // own adds up.  (A block that adds up waits for the prefix, and would hold its place from the blocks that have not begun.)  0: none.
     int own_parts;
 
-    LCU_HD long long first_cta(long long pair) const { return pair * key_tiles / per; }
-    LCU_HD long long last_cta(long long pair) const { return ((pair + 1) * key_tiles - 1) / per; }
-    LCU_HD long long slots() const { return ctas + pairs; }
+    LCU_HD int head_cost() const { return ((row_tiles - 1) * cost + cost_last) * key_tiles; }
+    // Cost of all units ahead of one; a CTA's units are those where this lies in its range.
+    LCU_HD int ahead(int pair, int tile) const {
+        const int h = pair / row_tiles, r = pair - h * row_tiles;
+        return h * head_cost() + r * cost * key_tiles + tile * (r + 1 < row_tiles ? cost : cost_last);
+    }
+    LCU_HD int unit_at(unsigned at) const {  // the first with that much ahead of it, or more
+        const int h = (int)(at / (unsigned)head_cost()), left = (int)(at - (unsigned)h * (unsigned)head_cost()), full = (row_tiles - 1) * key_tiles;
+        if (h >= pairs / row_tiles) return units;
+        const int u = h * row_tiles * key_tiles + (left <= full * cost ? (left + cost - 1) / cost : full + (left - full * cost + cost_last - 1) / cost_last);
+        return u < units ? u : units;
+    }
+    LCU_HD int first_cta(int pair) const { return ahead(pair, 0) / per; }
+    LCU_HD int last_cta(int pair) const { return ahead(pair, key_tiles - 1) / per; }
+    LCU_HD int slots() const { return ctas + pairs; }
 };
 
 // Number of (KV head, row tile) pairs of n tokens, `group` query heads per KV head; parts of a row's own slots.
@@ -58,7 +71,12 @@ inline bool prefix_walk(int n, int group, int nkvh, uint32_t prefix_len, long lo
     return (steps > bytes ? steps : bytes) < 2.5 + dh / 32 + (prefix_own_parts(n, nkvh, sms) ? 3.0 * dh / 128 : 0) + tiles;
 }
 
-// A prefix of prefix_len > 0 positions, at most `sms` CTAs; own_slots: what the sequences' own tables have room for.
+// Costs and units are counted in 32 bits, which is more than two seconds of work.
+inline bool prefix_fits(int n, int group, int nkvh, uint32_t prefix_len) {
+    return prefix_pairs(n, group, nkvh) <= 0x10000000 && prefix_pairs(n, group, nkvh) * ((prefix_len + (long long)PF_TILE - 1) / PF_TILE) <= 0x10000000;
+}
+
+// A prefix of prefix_len > 0 positions (that prefix_fits), at most `sms` CTAs; own_slots: what the sequences' own tables have room for.
 // One CTA of the prefix fills an SM.  The own slots' blocks get the SMs that it leaves, and all of them behind it: fewer CTAs of the prefix
 // with more key tiles each make it longer and the rest shorter.  Estimates in microseconds: 8 to begin and end, a key tile 1.2 to 2.4 (heads
 // of 0 to 128), 7 from a piece to the next, own slots (half of what there is room for) at 30 KB per SM.
@@ -67,24 +85,30 @@ inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, i
     p.rows = n * group;
     p.row_tiles = (p.rows + PF_ROWS - 1) / PF_ROWS;
     p.key_tiles = (int)((prefix_len + PF_TILE - 1) / PF_TILE);
-    p.pairs = prefix_pairs(n, group, nkvh);
+    p.pairs = (int)prefix_pairs(n, group, nkvh);
     p.units = p.pairs * p.key_tiles;
     p.slot_rows = p.rows < PF_ROWS ? p.rows : PF_ROWS;
     p.own_parts = prefix_own_parts(n, nkvh, sms);
-    const double tile = 1.2 + 1.2 * dh / 128, own = (double)nkvh * own_slots * dh * 4 * 0.5 / 30e3;  // the latter in SM microseconds
-    const long long least = (p.units + sms - 1) / sms;
+    const int last = p.rows - (p.row_tiles - 1) * PF_ROWS;  // rows of the last row tile
+    const bool uneven = p.row_tiles > 1 && last <= 128;
+    p.cost = uneven ? 3 : 1;
+    p.cost_last = uneven ? 2 : 1;
+    const int total = nkvh * p.head_cost();
+    const long long pair_cost = (long long)p.key_tiles * p.cost;
+    const double tile = (1.2 + 1.2 * dh / 128) * (p.row_tiles == 1 && last <= 128 ? 0.7 : 1) / p.cost, own = (double)nkvh * own_slots * dh * 4 * 0.5 / 30e3;  // the latter in SM microseconds
+    const long long fair = ((long long)total + sms - 1) / sms, least = fair < p.cost ? p.cost : fair;  // no range without a unit
     double best = 0;
-    for (long long per = least; per <= 8 * least && per <= p.units; ++per) {
-        const long long ctas = (p.units + per - 1) / per;
-        const long long pieces = per >= p.key_tiles ? (per + p.key_tiles - 1) / p.key_tiles : p.key_tiles % per ? 2 : 1;
+    for (long long per = least; per <= 8 * least && (per == least || per <= total); ++per) {
+        const long long ctas = (total - p.cost_last) / per + 1;
+        const long long pieces = per >= pair_cost ? (per + pair_cost - 1) / pair_cost : pair_cost % per ? 2 : 1;
         const double prefix = 1 + 7 * pieces + tile * per, left = p.own_parts ? own - (double)(sms - ctas) * (prefix - 8) : 0;
         const double t = prefix + (left > 0 ? left / sms + (left < 4.0 * sms ? left * 1.5 / sms : 6) : 0);
         if (per == least || t < best) {
             best = t;
-            p.per = per;
+            p.per = (int)per;
             p.ctas = (int)ctas;
         }
-        if (!p.own_parts || per > least + 64) break;
+        if (!p.own_parts || per > least + 64 * p.cost) break;
     }
     return p;
 }

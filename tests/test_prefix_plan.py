@@ -18,11 +18,22 @@ int main() {
     long long own;
     while (scanf("%d %d %d %u %d %d %lld", &n, &group, &nkvh, &len, &sms, &dh, &own) == 7) {
         const lcu::PrefixPlan p = lcu::prefix_plan(n, group, nkvh, len, sms, dh, own);
-        printf("%lld %lld %lld %d %d %d %d %zu %zu %zu", p.pairs, p.units, p.per, p.ctas, p.key_tiles, p.slot_rows, p.own_parts, lcu::prefix_own_row(p),
+        printf("%d %d %d %d %d %d %d %zu %zu %zu", p.pairs, p.units, p.per, p.ctas, p.key_tiles, p.slot_rows, p.own_parts, lcu::prefix_own_row(p),
                lcu::prefix_ml_bytes(p, nkvh) + lcu::prefix_part_rows(p, nkvh) * dh * 4, lcu::prefix_bytes(n, group, nkvh, len, sms, dh));
+        bool dealt = p.unit_at(0) == 0 && p.unit_at(p.ctas * p.per) == p.units;
+        for (long long c = 0, pair = 0; c < p.ctas; ++c) {  // every CTA has units, all of them its own, and none is left out
+            const long long u0 = p.unit_at(c * p.per), u1 = p.unit_at((c + 1) * p.per);
+            dealt = dealt && u0 < u1;
+            for (long long u = u0; u < u1 && p.units < 100000; u = (pair + 1) * p.key_tiles < u1 ? (pair + 1) * p.key_tiles : u1) {
+                pair = u / p.key_tiles;
+                const long long end = (pair + 1) * p.key_tiles < u1 ? (pair + 1) * p.key_tiles : u1;
+                dealt = dealt && p.first_cta(pair) <= c && c <= p.last_cta(pair) && p.ahead(pair, u - pair * p.key_tiles) / p.per == c &&
+                        p.ahead(pair, end - 1 - pair * p.key_tiles) / p.per == c;
+            }
+        }
         const long long show = p.pairs < 5000 ? p.pairs : 5000;
-        for (long long i = 0; i < show; ++i) printf(" %lld %lld", p.first_cta(i), p.last_cta(i));
-        printf(" %d %d\n", lcu::prefix_walk(n, group, nkvh, len, own, sms, dh), lcu::own_splits((long long)n * nkvh, own + len, sms));
+        for (long long i = 0; i < show; ++i) printf(" %d %d", p.first_cta(i), p.last_cta(i));
+        printf(" %d %d %d %d\n", dealt, p.cost, lcu::prefix_walk(n, group, nkvh, len, own, sms, dh), lcu::own_splits((long long)n * nkvh, own + len, sms));
     }
 }
 """
@@ -48,13 +59,20 @@ def test_every_unit_belongs_to_one_cta_and_every_piece_has_a_slot(plans):
     for shape, p in zip(SHAPES, plans(SHAPES)):
         n, group, nkvh, length, _, _ = shape
         pairs, units, per, ctas, key_tiles, slot_rows, parts, own_row, used, bound = p[:10]
-        ends = list(zip(p[10:-2:2], p[11:-2:2]))
+        ends = list(zip(p[10:-4:2], p[11:-4:2]))
         assert key_tiles == -(-length // 128) and pairs == nkvh * -(-n * group // 256) and units == pairs * key_tiles, shape
-        assert 1 <= ctas <= SMS and (ctas - 1) * per < units <= ctas * per, shape  # every CTA has units: none meets a range that is empty
+        assert 1 <= ctas <= SMS and p[-4] == 1, shape
+        last = n * group - (n * group - 1) // 256 * 256
+        cost, cost_last = (3, 2) if n * group > 256 and last <= 128 else (1, 1)
+        assert p[-3] == cost
+        starts, at = [], 0
+        for pair in range(len(ends)):
+            starts.append(at)
+            at += key_tiles * (cost_last if (pair + 1) % (pairs // nkvh) == 0 else cost)
         slots = set()
         for pair, (first, last) in enumerate(ends):
-            lo, hi = pair * key_tiles, (pair + 1) * key_tiles
-            assert first * per <= lo < (first + 1) * per and last * per < hi <= (last + 1) * per, shape
+            end = starts[pair + 1] if pair + 1 < len(starts) else at
+            assert first == starts[pair] // per and starts[pair] // per <= last <= (end - 1) // per, shape
             for cta in range(first, last + 1):
                 assert cta + pair not in slots, shape
                 slots.add(cta + pair)
@@ -69,9 +87,10 @@ def test_parts_of_own_slots(plans):
 
 
 def test_the_largest_call(plans):
-    shape = (65535, 16, 65535, 2 ** 31 - 1, 128, 65535 * (2 ** 31 - 1))
-    p = plans([shape])[0]
-    assert p[1] == 65535 * 4096 * 2 ** 24 and p[3] * p[2] >= p[1] > (p[3] - 1) * p[2]
+    """2^28 units: costs of 3 each still fit."""
+    for shape in [(4096, 16, 256, 128 * 4096, 128, 0), (4100, 16, 8, 128 * 130500, 128, 0), (65535, 16, 65535, 1, 128, 0)]:
+        p = plans([shape])[0]
+        assert p[1] <= 2 ** 28 < 2 * p[1] and p[-4] == 1 and 1 <= p[3] <= SMS
 
 
 def source(name):

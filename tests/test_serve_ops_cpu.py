@@ -139,3 +139,8 @@ def test_counts_whose_indices_would_not_fit(L):
     refused(L, append(L, n=2 ** 30 + 1), "tokens")
     size = L.load_library().lcu_attention_prefix_workspace_size
     assert size(65536, 8, 2, 128, 100) == size(2 ** 31 - 1, 2 ** 31 - 1, 1, 128, 2 ** 32 - 1) == size(3, 34, 2, 128, 100) == 0  # (what the call refuses)
+
+
+def test_more_units_than_a_call_takes(L):
+    refused(L, attention(L, n=65535, nh=64, nkvh=8, prefix=2 ** 31 - 1, stride=0), "more than a call takes")
+    assert L.load_library().lcu_attention_prefix_workspace_size(65535, 64, 8, 128, 2 ** 31 - 1) == 0
