@@ -7,8 +7,12 @@
 // all in 32 bits with one rounding at the end.  Every row is read once and written once, so HBM is the floor; what has to be kept down
 // on the way there is instructions and waits.  heads_kernel: a row is held by dh / 16 lanes, each with 8 values of the lower half and the
 // 8 that stand dh / 2 behind them, so that the pairs of either kind meet in one thread; lanes stay with their head from token to token
-// and request the next token's row while they work on one.  rows_kernel takes what heads_kernel cannot (halves of
-// a part of the head), rows_any_kernel the rest (sizes, strides or addresses that are no multiples of 16 bytes).
+// and request the next token's row while they work on one.  rows_kernel takes heads of an
+// odd number of pieces (dh 72, 40, ..), rows_any_kernel the rest (sizes, strides or addresses that are no multiples of 16 bytes).
+//
+// Measured on a B200: 8000 tokens of 32 + 8 heads of 64 (bf16, pairs side by side, 83 MB) 22.6 us, 3.7 TB/s, where adding a number to as many
+// values takes 16.2; 8004 tokens of 32 + 8 + 8 heads of 128 with norms into pages (halves, 201 MB) 43.7 us, 4.6 TB/s of 32.8; one token 5 us, which
+// is launch and three round trips.
 #include "paged.cuh"
 
 #include <mutex>
@@ -139,13 +143,15 @@ __device__ __forceinline__ unsigned long long rw_mul2(unsigned long long x, unsi
     return r;
 }
 
-// LPR lanes hold a row of dh <= 16 LPR values, each 8 from 8 c and 8 from dh / 2 + 8 c on.  HALVES: rot == dh, pairs (i, i + dh / 2).
-// Otherwise pairs (2 i, 2 i + 1).  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every gridDim.x-th token.
+// LPR lanes hold a row of dh <= 16 LPR values, each 8 from d on and 8 from d + gap on.  HALVES: pairs (i, i + rot / 2), so gap is rot / 2 in the
+// rotated part and half of the rest behind it.  Otherwise pairs (2 i, 2 i + 1), and gap is dh / 2.  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every gridDim.x-th token.
 template <class T, int LPR, bool HALVES, bool WF>
 __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) heads_kernel(const RowsArgs a, int n, int rows_per) {
     const int c = threadIdx.x % LPR, local = threadIdx.x / LPR, r = blockIdx.y * rows_per + local, total = a.nh + a.nkvh + a.n_v;
-    const int lower = a.dh / 2, d = 8 * c;
-    const bool in = d < lower && local < rows_per && r < total, is_q = r < a.nh, is_v = r >= a.nh + a.nkvh;
+    const int half = a.rot >> 1;
+    const bool front = !HALVES || 8 * c < half;
+    const int gap = !HALVES ? a.dh / 2 : front ? half : (a.dh - a.rot) / 2, d = front ? 8 * c : a.rot + 8 * c - half;
+    const bool in = 8 * c < a.dh / 2 && local < rows_per && r < total, is_q = r < a.nh, is_v = r >= a.nh + a.nkvh;
     // where this lane reads and writes for token 0; from token to token, or by the token's place in the pages
     const T *src = in ? rw_src<T>(a, 0, r) + d : nullptr;
     T *dst = in ? rw_dst<T>(a, 0, r, 0) + d : nullptr;
@@ -156,11 +162,10 @@ __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) he
     Row8<T> g0, g1;                                               // this head's weights (f32 ones are read from L1 each time)
     if (w && !WF) {
         g0.load(reinterpret_cast<const T *>(w) + d);
-        g1.load(reinterpret_cast<const T *>(w) + lower + d);
+        g1.load(reinterpret_cast<const T *>(w) + gap + d);
     }
-    const int half = a.rot >> 1;
-    const bool turn0 = in && !is_v && d < a.rot, turn1 = in && !is_v && lower + d < a.rot;
-    const int at0 = HALVES ? d : d >> 1, at1 = HALVES ? d + 4 : (lower + d) >> 1;  // of a row of the tables
+    const bool turn0 = in && !is_v && (HALVES ? front : d < a.rot), turn1 = in && !is_v && (HALVES ? front : gap + d < a.rot);
+    const int at0 = HALVES ? d : d >> 1, at1 = HALVES ? d + 4 : (gap + d) >> 1;  // of a row of the tables
     const float inv_dh = 1.f / (float)a.dh;
     // Rows of the next tokens on their way into shared memory, each thread's own: [stage][16-byte piece][thread].
     constexpr int PIECES = (int)sizeof(T), HALF = PIECES / 2;  // 16 values
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) he
             const T *p = src + (size_t)tok * src_step;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const T *q = p + (i < HALF ? 0 : lower) + i % HALF * (16 / (int)sizeof(T));
+                const T *q = p + (i < HALF ? 0 : gap) + i % HALF * (16 / (int)sizeof(T));
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(&ring[stage][i][threadIdx.x])), "l"(q) : "memory");
             }
         }
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) he
                     if (WF) {
                         Row8<float> y0, y1;
                         y0.load(reinterpret_cast<const float *>(w) + d);
-                        y1.load(reinterpret_cast<const float *>(w) + lower + d);
+                        y1.load(reinterpret_cast<const float *>(w) + gap + d);
                         y0.get(g);
                         y1.get(h);
                     } else {
@@ -279,7 +284,7 @@ __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) he
         if (!in) continue;
         T *p = dst + (paged ? off : (size_t)t * dst_step);
         x0.store(p);
-        x1.store(p + lower);
+        x1.store(p + gap);
     }
 }
 
@@ -455,7 +460,9 @@ static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
         LCU_CHECK_CUDA(cudaGetLastError());
         return LCU_OK;
     }
-    if (a.dh % 16 == 0 && (!a.halves || a.rot == 0 || a.rot == a.dh)) {
+    // (Halves are in pieces of 8 where rot is a multiple of 16, which `vec` says.)  4000 tokens of 32 + 8 + 8 heads of 128 with norms, rot 64 by halves: 25.9
+    // us here, 35 in rows_kernel; heads of 80 with rot 40 by halves, whose pieces begin off 16 bytes, 82 in rows_any_kernel.
+    if (a.dh % 16 == 0) {
         const int lanes = a.dh / 16;
         return lanes <= 2 ? heads_form<T, 2>(a, n, s) : lanes <= 4 ? heads_form<T, 4>(a, n, s) : lanes <= 8 ? heads_form<T, 8>(a, n, s) : heads_form<T, 16>(a, n, s);
     }

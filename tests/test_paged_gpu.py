@@ -161,3 +161,12 @@ def test_append_behind_32_bits(L):
     assert torch.equal(pool[pages - 1, 0, :, 5], k[0]) and torch.equal(pool[0, 1, :, 2], v[1])
     assert torch.equal(pool[pages - 1, 1, :, 5], v[0]) and torch.equal(pool[0, 0, :, 2], k[1])
     assert not pool[1:pages - 1].any()
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2])
+@pytest.mark.parametrize("dh,rot", [(128, 64), (128, 16), (128, 112), (64, 48), (32, 16), (96, 32), (256, 240), (192, 96), (16, 16), (16, 0),
+                                    (8, 0), (24, 16), (40, 32), (72, 48), (72, 64), (104, 16), (248, 240)])
+@pytest.mark.parametrize("n", [3, 1200])
+def test_rotations_of_a_part_of_the_head(L, dt, dh, rot, n):
+    test_norm_and_rotation(L, dt, n, 5, 2, dh, rot, True, "own", "whole")
+    test_norm_and_rotation(L, dt, n, 5, 2, dh, rot - 8 if rot > 8 else rot, False, "f32", "cut")
