@@ -39,6 +39,9 @@ template <> __device__ __forceinline__ float vf_f<float>(float v) { return v; }
 // CTA requests its part of the next row (one bulk copy into shared memory) as soon as it has taken up this one: the memory works on
 // while maxima, exponentials and sums wait for one another.
 //
+// Measured on a B200, f32: 160 rows of 128256 33.4 us, 4.9 TB/s (adding a number to as many values takes 27.6); 300 of 50257 30.8; 76 of 262144 55.5
+// with 1024 threads (73 when they were read twice); one f16 row of 32000 3.7, which is launch and four round trips.
+//
 // Rows of any stride: where the strides of logits and probabilities agree modulo a 16-byte piece, a row is taken from the piece on that it begins
 // in, and what lies ahead of it in that piece counts as -inf and is not written.
 struct SoftmaxArgs {
@@ -323,6 +326,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
 // in 64 bits, where the products u q and the differences of 32-bit numbers are exact.  Bound by HBM: of all rows only the pair that the last token is drawn
 // from is read whole.  A cluster of up to 8 CTAs takes a sequence: sums of pieces of 512 values or more, totals across the cluster
 // in one exchange, and the CTA that the threshold falls into reads the one piece that holds it again.  The order of the sums is fixed.
+// Measured on a B200, f32: 64 sequences of 128256 tokens 21 us (66 MB; a plain sum of 82 MB takes 22.3), 30 where rows begin off 16 bytes; one sequence of
+// 32000 6.5, a chain of drafts, gathers, row, cluster and piece.
 struct VerifyArgs {
     int32_t *accepted, *tokens;
     const void *target, *draft;
