@@ -1,5 +1,8 @@
 """Attention of a batch that shares a prefix, on a caller's pages (needs a B200)."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -435,3 +438,64 @@ def test_own_contexts_of_few_and_many_blocks(L, dh, nh, nkvh, tokens, own):
     b = Batch(dh + tokens, [(1 + (own * (i + 1)) // tokens, 1) for i in range(tokens)], 0 if tokens > 20 else 70, nh, nkvh, dh, 1, 16)
     b.run(L)
     b.check()
+
+
+FIRST = """
+import sys
+sys.path[:0] = sys.argv[1:3]
+import torch
+import llama_cu_b200 as L
+import serve_ref as R
+import test_prefix_gpu as P
+lib = L.load_library()
+few, many = P.Batch(1, [(5, 1), (40, 2)], 100, 32, 8, 128, 0, 16), P.Batch(2, [(30, 1)] * 40, 3000, 32, 8, 128, 1, 64)
+x = R.rng_normal(3, (400, 20001), 2)
+probs = torch.zeros_like(x)
+u = torch.rand(100, 4, device="cuda")
+drafted = torch.zeros(100, 3, dtype=torch.int32, device="cuda")
+accepted, tokens = torch.zeros(100, dtype=torch.int32, device="cuda"), torch.zeros(100, 4, dtype=torch.int32, device="cuda")
+q = R.rng_normal(4, (50, 8, 128), 0)
+out, pos = torch.zeros_like(q), torch.arange(50, dtype=torch.int32, device="cuda")
+sin, cos = R.tables(50, 64)
+prep = L.QkPrep(None, None, sin.data_ptr(), cos.data_ptr(), 0, 1e-6, 50, 64, 1)
+slots = torch.arange(50, dtype=torch.int32, device="cuda")
+seq, table = torch.zeros_like(slots), torch.arange(4, dtype=torch.int32, device="cuda")
+pool = torch.zeros(4, 2, 8, 16, 128, dtype=torch.float16, device="cuda")
+pages = L.KvPages(pool.data_ptr(), pool[:, 1].data_ptr(), pool.stride(0), pool.stride(3), pool.stride(2), 4, 16)
+for b in (few, many):
+    b.dev = [R.i32(b.prefix_ids), R.i32(b.ids), R.i32(b.tok_seq), R.i32(b.ctx)]
+    b.ws = torch.zeros(lib.lcu_attention_prefix_workspace_size(b.n, 32, 8, 128, b.prefix), dtype=torch.uint8, device="cuda")
+
+def calls():
+    s = R.stream()
+    L.check(lib.lcu_op_qk_norm_rope(out.data_ptr(), 1024, 128, q.data_ptr(), 1024, 128, None, 0, 0, None, 0, 0, pos.data_ptr(), prep, 50, 8, 0, 128, 0, s))
+    L.check(lib.lcu_op_kv_append(pages, table.data_ptr(), 4, 1, seq.data_ptr(), slots.data_ptr(), q.data_ptr(), 1024, 128, out.data_ptr(), 1024, 128, None, 0, 0, None, 0, 0,
+                                 None, None, 50, 0, 8, 128, 0, s))
+    for b in (few, many):
+        L.check(lib.lcu_op_attention_prefix(b.o.data_ptr(), b.o.stride(0), 128, b.q.data_ptr(), b.q.stride(0), 128, L.KvPages(*b.pages_args()), b.dev[0].data_ptr(), b.prefix,
+                                            b.dev[1].data_ptr(), b.per, b.n_seq, b.dev[2].data_ptr(), b.dev[3].data_ptr(), b.n, 32, 8, 128, b.scale, b.dims[3],
+                                            b.ws.data_ptr(), b.ws.numel(), s))
+    L.check(lib.lcu_op_softmax_rows(probs.data_ptr(), 20001, x.data_ptr(), 20001, None, 400, 20001, 2, s))
+    L.check(lib.lcu_op_verify_drafts(accepted.data_ptr(), tokens.data_ptr(), probs.data_ptr(), 20001, None, 0, drafted.data_ptr(), None, u.data_ptr(), 100, 3, 20001, 2, s))
+
+torch.cuda.synchronize()
+graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(graph, stream=side):
+    calls()  # nothing of the library has run before
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (out, pool, few.o, many.o, probs, accepted, tokens)]
+few.check(), many.check()
+for t in (out, pool, few.o, many.o, probs, accepted, tokens):
+    t.zero_()
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (out, pool, few.o, many.o, probs, accepted, tokens))) and got[1].any()
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(L):
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(here), here], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
