@@ -258,24 +258,28 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         const int t = (warp - 2) >> 2, q = warp & 3, row = q * 32 + lane;  // a warp may only touch TMEM lanes [32 q, 32 q + 32)
         const int group = a.nh / a.nkvh;
         const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + 128 * t, to = tmem_o + ((uint32_t)(q * 32) << 16) + DH * t;
-        auto load_q = [&](const PfPiece &p) {  // 16 bytes per thread and step, as the 128-byte swizzle has them; zeros behind the last row
-            constexpr int CH = DH / 8;
-            const int i = tid - 64 - 128 * t, c = i % CH;
-            uint4 u[CH];
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const int at = 128 * t + i / CH + k * (128 / CH);
-                u[k] = make_uint4(0, 0, 0, 0);
-                if (at < p.rows) {
-                    const int tok = (p.row0 + at) / group, g = p.row0 + at - tok * group;
-                    u[k] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + (size_t)tok * a.stq + (size_t)(p.hkv * group + g) * a.shq + 8 * c);
+        // 16 bytes per thread and step, as the 128-byte swizzle has them; zeros behind the last row.  A short loop of asynchronous copies: unrolled,
+        // with the rows in registers, it was the longest part of a cold start (4 of 5 us).
+        auto load_q = [&](const PfPiece &p) {
+            constexpr int CH = DH / 8, STEP = 128 / CH;  // rows a step
+            const int i = tid - 64 - 128 * t, c = i % CH, r0 = i / CH, left = p.rows - 128 * t;
+            int tok = (p.row0 + 128 * t + r0) / group, g = p.row0 + 128 * t + r0 - tok * group;
+            const int tok_step = STEP / group, g_step = STEP - tok_step * group;
+            uint32_t dst = tc_smem(Qs) + (uint32_t)(t * TILE + (c >> 3) * AT_BOX + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4));
+#pragma unroll 1
+            for (int r = r0; r < 128; r += STEP) {
+                const bool valid = r < left;
+                const T *src = reinterpret_cast<const T *>(a.q) + (valid ? (size_t)tok * a.stq + (size_t)(p.hkv * group + g) * a.shq + 8 * c : 0);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+                dst += STEP * 128;
+                tok += tok_step;
+                g += g_step;
+                if (g >= group) {
+                    g -= group;
+                    ++tok;
                 }
             }
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const int r = i / CH + k * (128 / CH);
-                *reinterpret_cast<uint4 *>(Qs + t * TILE + (c >> 3) * AT_BOX + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = u[k];
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             pf_arrive(tc_smem(&sh->q_full[t]), lane);
         };
