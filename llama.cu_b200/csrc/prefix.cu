@@ -547,19 +547,22 @@ __global__ void __launch_bounds__(OW_THREADS, DEPTH == 1 ? 8 : 5) own_kernel(con
     const bool leave = a.prefix_len && a.plan.own_parts, cluster = splits > 1 && !leave;
     if (cluster) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of stores to the first CTA
     // consecutive tokens of one sequence, cut at multiples of tokens_per
-    const int seq = a.tok_seq[t];
-    const bool mine = seq >= 0 && seq < a.n_seq && (t % tokens_per == 0 || a.tok_seq[t - 1] != seq);
+    // (of all tokens that may be among them, in one round trip)
+    const int before = t % tokens_per, most = min(tokens_per - before, a.n - t);
+    const int lane_seq = a.tok_seq[t + min(lane, most - 1)], last_seq = before ? a.tok_seq[t - 1] : -1;
+    const uint32_t lane_ctx = a.tok_ctx[t + min(lane, most - 1)];
+    const int seq = __shfl_sync(0xffffffffu, lane_seq, 0);
+    const bool mine = seq >= 0 && seq < a.n_seq && (before == 0 || last_seq != seq);
     if (!mine) {
         if (cluster) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         if (first_block) grid_dep_wait();  // the grid ends behind the prefix, whatever its blocks have to do
         return;
     }
-    const int most = min(tokens_per - t % tokens_per, a.n - t);
-    const unsigned same = __ballot_sync(0xffffffffu, lane < most && a.tok_seq[t + min(lane, most - 1)] == seq);
+    const unsigned same = __ballot_sync(0xffffffffu, lane < most && lane_seq == seq);
     const int n_tok = __ffs(~same) - 1, rows = n_tok * group;  // most <= 16: there is a zero
     const uint32_t cap = (uint32_t)a.table_stride << a.page_shift;
     uint32_t ctx = 0;  // of the longest
-    if (lane < n_tok) ctx = min(a.tok_ctx[t + lane], cap);
+    if (lane < n_tok) ctx = min(lane_ctx, cap);
     const int r0 = gid, r1 = gid + 8;  // this thread's rows
     const uint32_t lim0 = __shfl_sync(0xffffffffu, ctx, r0 / group), lim1 = __shfl_sync(0xffffffffu, ctx, r1 / group);  // 0 behind the last row
     const uint32_t lim_min = __reduce_min_sync(0xffffffffu, lane < n_tok ? ctx : 0xffffffffu);
