@@ -59,16 +59,17 @@ inline int own_splits(long long blocks, long long slots, int sms) {
 }
 
 // A prefix that the blocks of the own slots read themselves, once per token, instead of the tensor cores once per 256 rows: one launch instead
-// of two or three.  Estimates in microseconds, of heads of 128 (and of 64): a warp's 16 slots 0.75 (0.55), an SM 60 KB of keys and values from L2; for
-// the tensor cores 6.5 (4.5) to begin, end and add up, 3 (1.5) more where a third kernel adds up, 2.4 (1.8) a round of key tiles.  Measured with 32
-// heads over 8 of 128, 1 / 8 / 33 tokens: prefix of 16 5.5 / 6.0 / 7.4 us against 12.2 / 12.9 / 16.8; of 1000 9.2 / 13.1 / 31 against 12.5 / 13.1 / 18.6;
-// of 4000 18 / 31 / 101 against 17 / 20 / 27.
+// of two or three.  Estimates in microseconds, of heads of 128 (and of 64): a warp's 16 slots 0.75 (0.55), an SM 60 KB of keys and values from L2, clusters
+// beyond what runs at once their rows' sums; for the tensor cores 4.6 to begin, end and add up, 0.5 more where a third kernel adds up, 2.4 (1.8) a
+// round of key tiles.  Measured with 32 heads over 8 of 128, 1 / 8 / 33 tokens: prefix of 16 5.5 / 6.1 / 7.2 us against 10.1 / 10.8 / 14.3; of 600 7.6 /
+// 10.6 / 21.8 against 10.5 / 11.1 / 15.3; of 2000 12.1 / 18.9 / 55 against 12.9 / 16.1 / 19.2; of 4000 18 / 31 / 101 against 15 / 18 / 23.
 inline bool prefix_walk(int n, int group, int nkvh, uint32_t prefix_len, long long own_slots, int sms, int dh) {
     const long long blocks = (long long)n * nkvh;
     const int splits = own_splits(blocks, own_slots + prefix_len, sms);
     const double steps = (double)prefix_len / (32.0 * splits) * (0.35 + 0.4 * dh / 128), bytes = (double)blocks * prefix_len * dh * 4 / (60e3 * sms);
     const double tiles = (double)prefix_pairs(n, group, nkvh) * ((prefix_len + PF_TILE - 1) / PF_TILE) / sms * (1.2 + 1.2 * dh / 128);
-    return (steps > bytes ? steps : bytes) < 2.5 + dh / 32 + (prefix_own_parts(n, nkvh, sms) ? 3.0 * dh / 128 : 0) + tiles;
+    const double crowd = blocks * splits > sms && splits > 1 ? 0.06 * group * splits : 0;
+    return (steps > bytes ? steps : bytes) + crowd < 4.6 + (prefix_own_parts(n, nkvh, sms) ? 0.5 : 0) + tiles;
 }
 
 // Costs and units are counted in 32 bits, which is more than two seconds of work.

@@ -129,7 +129,7 @@ def test_a_softmax_whose_wait_ran_out_is_nan_and_leaves_after_its_copy():
 def test_a_prefix_is_read_by_the_blocks_of_the_own_slots_while_that_is_short(plans):
     def walks(n, length, group=4, nkvh=8, dh=128, own=100):
         return plans([(n, group, nkvh, length, dh, own)])[0][-2]
-    for n, short, long in ((1, 2000, 4000), (8, 1000, 2000), (33, 300, 1000), (100, 100, 300)):  # both measured
+    for n, short, long in ((1, 2000, 4000), (8, 600, 1000), (33, 100, 300), (100, 100, 300)):  # both measured
         assert walks(n, short) and not walks(n, long), n
     for n in (1, 3, 8, 33, 100, 1000, 20000):  # once too long, always
         kinds = [walks(n, length) for length in (1, 8, 16, 100, 500, 1000, 2000, 4000, 8000, 32000, 2 ** 31 - 1)]
