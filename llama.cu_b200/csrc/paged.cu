@@ -143,14 +143,19 @@ __device__ __forceinline__ unsigned long long rw_mul2(unsigned long long x, unsi
     return r;
 }
 
-// LPR lanes hold a row of dh <= 16 LPR values, each 8 from d on and 8 from d + gap on.  HALVES: pairs (i, i + rot / 2), so gap is rot / 2 in the
-// rotated part and half of the rest behind it.  Otherwise pairs (2 i, 2 i + 1), and gap is dh / 2.  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every gridDim.x-th token.
-template <class T, int LPR, bool HALVES, bool WF>
+// How values are paired: (2 i, 2 i + 1); (i, i + rot / 2) of a whole head, rot == dh or 0; the same of a part of it.
+enum { SIDE_BY_SIDE, HALVES_WHOLE, HALVES_PART };
+
+// LPR lanes hold a row of dh <= 16 LPR values, each 8 from d on and 8 from d + gap on: gap is dh / 2 or, in HALVES_PART, half of the rotated part or half
+// of the rest (46.7 us where HALVES_WHOLE has 43.7).  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every
+// gridDim.x-th token.
+template <class T, int LPR, int MODE, bool WF>
 __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) heads_kernel(const RowsArgs a, int n, int rows_per) {
     const int c = threadIdx.x % LPR, local = threadIdx.x / LPR, r = blockIdx.y * rows_per + local, total = a.nh + a.nkvh + a.n_v;
+    constexpr bool HALVES = MODE != SIDE_BY_SIDE, PART = MODE == HALVES_PART;
     const int half = a.rot >> 1;
-    const bool front = !HALVES || 8 * c < half;
-    const int gap = !HALVES ? a.dh / 2 : front ? half : (a.dh - a.rot) / 2, d = front ? 8 * c : a.rot + 8 * c - half;
+    const bool front = !PART || 8 * c < half;
+    const int gap = !PART ? a.dh / 2 : front ? half : (a.dh - a.rot) / 2, d = front ? 8 * c : a.rot + 8 * c - half;
     const bool in = 8 * c < a.dh / 2 && local < rows_per && r < total, is_q = r < a.nh, is_v = r >= a.nh + a.nkvh;
     // where this lane reads and writes for token 0; from token to token, or by the token's place in the pages
     const T *src = in ? rw_src<T>(a, 0, r) + d : nullptr;
@@ -164,7 +169,7 @@ __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) he
         g0.load(reinterpret_cast<const T *>(w) + d);
         g1.load(reinterpret_cast<const T *>(w) + gap + d);
     }
-    const bool turn0 = in && !is_v && (HALVES ? front : d < a.rot), turn1 = in && !is_v && (HALVES ? front : gap + d < a.rot);
+    const bool turn0 = in && !is_v && (PART ? front : d < a.rot), turn1 = in && !is_v && (PART ? front : gap + d < a.rot);
     const int at0 = HALVES ? d : d >> 1, at1 = HALVES ? d + 4 : (gap + d) >> 1;  // of a row of the tables
     const float inv_dh = 1.f / (float)a.dh;
     // Rows of the next tokens on their way into shared memory, each thread's own: [stage][16-byte piece][thread].
@@ -428,7 +433,7 @@ static int rows_launch(const RowsArgs &a, int n, cudaStream_t s) {
     return LCU_OK;
 }
 
-template <class T, int LPR, bool HALVES, bool WF>
+template <class T, int LPR, int MODE, bool WF>
 static int heads_launch(const RowsArgs &a, int n, cudaStream_t s) {
     // blocks of up to 128 threads with an even part of a token's rows; as many as run at once
     const int rows = a.nh + a.nkvh + a.n_v, parts = (rows * LPR + HK_THREADS - 1) / HK_THREADS, per = (rows + parts - 1) / parts, threads = (per * LPR + 31) / 32 * 32;
@@ -438,18 +443,23 @@ static int heads_launch(const RowsArgs &a, int n, cudaStream_t s) {
     {
         std::lock_guard<std::mutex> lk(mu);
         int &have = resident[threads / 32];
-        if (!have) LCU_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&have, heads_kernel<T, LPR, HALVES, WF>, threads, 0));
+        if (!have) LCU_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&have, heads_kernel<T, LPR, MODE, WF>, threads, 0));
         blocks = have * sm_count() / parts;
     }
-    heads_kernel<T, LPR, HALVES, WF><<<dim3(n < blocks || blocks < 1 ? n : blocks, parts), threads, 0, s>>>(a, n, per);
+    heads_kernel<T, LPR, MODE, WF><<<dim3(n < blocks || blocks < 1 ? n : blocks, parts), threads, 0, s>>>(a, n, per);
     LCU_CHECK_CUDA(cudaGetLastError());
     return LCU_OK;
 }
+template <class T, int LPR, int MODE>
+static int heads_mode(const RowsArgs &a, int n, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (a.w_f32) return heads_launch<T, LPR, MODE, true>(a, n, s);
+    return heads_launch<T, LPR, MODE, false>(a, n, s);
+}
 template <class T, int LPR>
 static int heads_form(const RowsArgs &a, int n, cudaStream_t s) {
-    if constexpr (sizeof(T) == 2)
-        if (a.w_f32) return a.halves ? heads_launch<T, LPR, true, true>(a, n, s) : heads_launch<T, LPR, false, true>(a, n, s);
-    return a.halves ? heads_launch<T, LPR, true, false>(a, n, s) : heads_launch<T, LPR, false, false>(a, n, s);
+    if (!a.halves) return heads_mode<T, LPR, SIDE_BY_SIDE>(a, n, s);
+    return a.rot == 0 || a.rot == a.dh ? heads_mode<T, LPR, HALVES_WHOLE>(a, n, s) : heads_mode<T, LPR, HALVES_PART>(a, n, s);
 }
 
 template <class T>
