@@ -925,7 +925,7 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
         a.walk_len = prefix_len;
         a.prefix_len = 0;
     } else if (prefix_len) {
-        a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh, (long long)(n_seq < n ? n_seq : n) * table_stride * pages->page_tokens);
+        a.plan = prefix_plan(n, nh / nkvh, nkvh, prefix_len, sm_count(), dh, (long long)(n_seq < n ? n_seq : n) * table_stride * pages->page_tokens, n_seq);
         a.part_ml = reinterpret_cast<float2 *>(workspace);
         a.part_o = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + prefix_ml_bytes(a.plan, nkvh));
         a.own_row = prefix_own_row(a.plan);

@@ -23,8 +23,8 @@ struct PrefixPlan {
     int pairs, units, per;        // (KV head, row tile); all units; cost of a CTA
     int ctas, cost, cost_last;    // of a unit; of one in a KV head's last row tile
     int slot_rows;   // rows of a piece's slot
-    // More (KV head, token) blocks for the own slots than SMs: they leave their parts too, at most so many of a row, and a kernel of its
-    // own adds up.  (A block that adds up waits for the prefix, and would hold its place from the blocks that have not begun.)  0: none.
+    // Parts of a row's own slots, at most, that the (KV head, token) blocks leave for a kernel of its own, which adds up with a warp per row.  0: the
+    // blocks add up themselves, one row after another.
     int own_parts;
 
     LCU_HD int head_cost() const { return ((row_tiles - 1) * cost + cost_last) * key_tiles; }
@@ -47,8 +47,8 @@ struct PrefixPlan {
 // Number of (KV head, row tile) pairs of n tokens, `group` query heads per KV head; parts of a row's own slots.
 inline long long prefix_pairs(int n, int group, int nkvh) { return (long long)nkvh * ((n * group + PF_ROWS - 1) / PF_ROWS); }
 inline int prefix_own_parts(int n, int nkvh, int sms) {
-    const long long blocks = (long long)n * nkvh;
-    return blocks <= sms ? 0 : blocks >= 3LL * sms ? 1 : (int)(3LL * sms / blocks);
+    const long long blocks = (long long)n * nkvh, parts = blocks >= 3LL * sms ? 1 : 3LL * sms / blocks;
+    return parts < 8 ? (int)parts : 8;
 }
 
 // CTAs that share a (KV head, token)'s slots and add up their parts as a cluster: up to 8 where blocks are few, 64 slots and more each.
@@ -69,7 +69,7 @@ inline bool prefix_walk(int n, int group, int nkvh, uint32_t prefix_len, long lo
     const double steps = (double)prefix_len / (32.0 * splits) * (0.35 + 0.4 * dh / 128), bytes = (double)blocks * prefix_len * dh * 4 / (60e3 * sms);
     const double tiles = (double)prefix_pairs(n, group, nkvh) * ((prefix_len + PF_TILE - 1) / PF_TILE) / sms * (1.2 + 1.2 * dh / 128);
     const double crowd = blocks * splits > sms && splits > 1 ? 0.06 * group * splits : 0;
-    return (steps > bytes ? steps : bytes) + crowd < 4.6 + (prefix_own_parts(n, nkvh, sms) ? 0.5 : 0) + tiles;
+    return (steps > bytes ? steps : bytes) + crowd < 4.6 + (blocks > sms ? 0.5 : 0) + tiles;
 }
 
 // Costs and units are counted in 32 bits, which is more than two seconds of work.
@@ -81,7 +81,7 @@ inline bool prefix_fits(int n, int group, int nkvh, uint32_t prefix_len) {
 // One CTA of the prefix fills an SM.  The own slots' blocks get the SMs that it leaves, and all of them behind it: fewer CTAs of the prefix
 // with more key tiles each make it longer and the rest shorter.  Estimates in microseconds: 8 to begin and end, a key tile 1.2 to 2.4 (heads
 // of 0 to 128), 7 from a piece to the next, own slots (half of what there is room for) at 30 KB per SM.
-inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, int sms, int dh, long long own_slots) {
+inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, int sms, int dh, long long own_slots, int n_seq = 0x7fffffff) {
     PrefixPlan p;
     p.rows = n * group;
     p.row_tiles = (p.rows + PF_ROWS - 1) / PF_ROWS;
@@ -89,7 +89,6 @@ inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, i
     p.pairs = (int)prefix_pairs(n, group, nkvh);
     p.units = p.pairs * p.key_tiles;
     p.slot_rows = p.rows < PF_ROWS ? p.rows : PF_ROWS;
-    p.own_parts = prefix_own_parts(n, nkvh, sms);
     const int last = p.rows - (p.row_tiles - 1) * PF_ROWS;  // rows of the last row tile
     const bool uneven = p.row_tiles > 1 && last <= 128;
     p.cost = uneven ? 3 : 1;
@@ -98,6 +97,13 @@ inline PrefixPlan prefix_plan(int n, int group, int nkvh, uint32_t prefix_len, i
     const long long pair_cost = (long long)p.key_tiles * p.cost;
     const double tile = (1.2 + 1.2 * dh / 128) * (p.row_tiles == 1 && last <= 128 ? 0.7 : 1) / p.cost, own = (double)nkvh * own_slots * dh * 4 * 0.5 / 30e3;  // the latter in SM microseconds
     const long long fair = ((long long)total + sms - 1) / sms, least = fair < p.cost ? p.cost : fair;  // no range without a unit
+    // More blocks than SMs do not add up: they would wait for the prefix and hold their places from those that have not begun.  Nor do blocks of
+    // many rows and parts: a warp takes every second row, and eight parts of it, in a microsecond, where the third kernel costs 2.5 (64 heads over
+    // 8, 2 x 5 drafted tokens behind 1391 26.5 us and 14.6 with it, 16 over 1, 3 x 5 behind 9000 64 and 25; 32 over 8, 3 tokens behind 8000, 6 rounds, 22.8
+    // and 25.2).
+    const long long each = ((long long)n + n_seq - 1) / n_seq, tokens = each < 16 / group ? each : 16 / group;  // of a block, about
+    const long long rounds = (pair_cost / least + 9) / 8 * ((tokens * group + 1) / 2);
+    p.own_parts = (long long)n * nkvh > sms || rounds > 6 ? prefix_own_parts(n, nkvh, sms) : 0;
     double best = 0;
     for (long long per = least; per <= 8 * least && (per == least || per <= total); ++per) {
         const long long ctas = (total - p.cost_last) / per + 1;
@@ -122,6 +128,7 @@ inline size_t prefix_ml_bytes(const PrefixPlan &p, int nkvh) { return (prefix_pa
 inline size_t prefix_bytes(int n, int group, int nkvh, uint32_t prefix_len, int sms, int dh) {
     PrefixPlan p = prefix_plan(n, group, nkvh, prefix_len, sms, dh, 0);
     p.ctas = sms;
+    p.own_parts = prefix_own_parts(n, nkvh, sms);
     return prefix_ml_bytes(p, nkvh) + prefix_part_rows(p, nkvh) * dh * 4;
 }
 
