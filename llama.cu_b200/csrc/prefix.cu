@@ -12,11 +12,11 @@
 //  - own_kernel: each token's own slots.  A CTA owns a KV head and up to 16 query rows of one sequence's consecutive tokens (drafted tokens
 //    share their keys); its two warps take 16 keys each in turns, with a softmax of their own and both products in registers (mma.sync),
 //    and meet once at the end.  It is launched as a programmatic dependent: its blocks run on the SMs that the prefix leaves, then on all.
-//  - The sum of all parts: at the end of own_kernel where its blocks are few, else in own_sum_kernel.
+//  - The sum of all parts: at the end of own_kernel where its blocks, their rows and the parts are few, else in own_sum_kernel.
 //  - A prefix that is short next to the number of tokens is read by own_kernel too, ahead of the token's own slots, and the call is one launch.
 //
-// Measured on a B200, heads of 128: 256 tokens of 64 heads over 8 behind 32000 positions 290 us (0.93 PFLOP/s; exponentials and products take
-// turns) and 344 in long runs at 1000 W; 16 x 5 drafted tokens of 32 over 8 behind 8001 37 us: prefix 24 (14 of units, 9 to begin, end and leave
+// Measured on a B200, heads of 128: 256 tokens of 64 heads over 8 behind 32000 positions 284 us (0.95 PFLOP/s; exponentials and products take
+// turns) and 341 in long runs at 1000 W; 16 x 5 drafted tokens of 32 over 8 behind 8001 35 us: prefix 22 (15 of units, 7 to begin, end and leave
 // parts), own slots 9, sum 4.
 //
 // f32 scores and softmax, sums in f32 over the weights as they are, weights rounded to the activation type ahead of the second product (its
