@@ -1,6 +1,7 @@
 // From logits to the tokens that a verified draft leaves (no counterpart in the reference, which samples one token per row,
 // exec/output_head.rs:104-113): probabilities of rows of logits, and the acceptance of drafted tokens against them.
 #include "paged.cuh"
+#include "row_exchange.hpp"
 #include "tc.cuh"
 
 namespace lcu {
@@ -39,8 +40,11 @@ template <> __device__ __forceinline__ float vf_f<float>(float v) { return v; }
 // CTA requests its part of the next row (one bulk copy into shared memory) as soon as it has taken up this one: the memory works on
 // while maxima, exponentials and sums wait for one another.
 //
-// Measured on a B200, f32: 160 rows of 128256 33.4 us, 4.9 TB/s (adding a number to as many values takes 27.6); 300 of 50257 30.8; 76 of 262144 55.5
-// with 1024 threads (73 when they were read twice); one f16 row of 32000 3.7, which is launch and four round trips.
+// Measured on a B200 (calls in a graph), f32: 160 rows of 128256 33.6 us, 4.9 TB/s (adding a number to as many values takes 27.6); 300 of 50257 28.5; 76 of
+// 262144 54.7 with 1024 threads (73 when they were read twice); bf16 logits, 160 of 128256 33.8; one f16 row of 32000 3.3, which is launch and four round trips.
+//
+// Waits are bounded.  A CTA whose wait has run out takes no further part (row_exchange.hpp): its values of that row and of those to come are NaN, and so are
+// those of peers that go without its maximum and sum.  The flag that says so is read ahead of each exchange, 0.5 % of long f32 rows and 2 % of 16-bit ones.
 //
 // Rows of any stride: where the strides of logits and probabilities agree modulo a 16-byte piece, a row is taken from the piece on that it begins
 // in, and what lies ahead of it in that piece counts as -inf and is not written.
@@ -82,6 +86,31 @@ __device__ __forceinline__ unsigned long long sm_key(float v, uint32_t i) {
     return ((unsigned long long)u << 32) | (uint32_t)~i;
 }
 
+// The steps of RowExchange on shared memory of the cluster's CTAs: 8 bytes into everyone's slot of this CTA, counted by their barriers.
+struct SoftmaxPort {
+    unsigned long long (*slots)[VF_CLUSTER], *bars, value;  // [turn][CTA], [turn]; what this CTA sends
+    volatile int *abort_flag;
+    uint32_t rank, size;
+    int tid;
+    __device__ __forceinline__ void started() const { vf_cluster_wait(); }
+    __device__ __forceinline__ void send(uint32_t turn) const {
+        if (tid == 0) tc_mbar_expect_tx(tc_smem(&bars[turn]), 8 * size);
+        if (tid < (int)size) vf_st_async(vf_peer(&slots[turn][rank], (uint32_t)tid), value, vf_peer(&bars[turn], (uint32_t)tid));
+    }
+    __device__ __forceinline__ bool wait(uint32_t turn, uint32_t parity) const { return tc_mbar_wait(tc_smem(&bars[turn]), parity, abort_flag); }
+    __device__ __forceinline__ bool gave_up() const { return *abort_flag != 0; }
+    __device__ __forceinline__ void give_up() const { *abort_flag = 1; }
+    __device__ __forceinline__ void together() const { __syncthreads(); }
+    __device__ __forceinline__ void others() const {  // (threads that have exited count as arrived)
+        vf_cluster_arrive();
+        vf_cluster_wait();
+    }
+    __device__ __forceinline__ void landed() const {  // far longer than a store takes
+        for (const unsigned long long t0 = tc_ns(); tc_ns() - t0 < TC_DRAIN_NS;) {
+        }
+    }
+};
+
 // grid (CTAs of a cluster, clusters); V values to a piece (1: rows are not in pieces of 16 bytes)
 template <class T, int V, int NT, int EPT, bool AHEAD>
 __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArgs a) {
@@ -91,11 +120,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
     __shared__ unsigned long long part[WARPS], xchg[2][VF_CLUSTER], xbar[2], bar;
     __shared__ float2 fpart[WARPS];
     __shared__ float spart[WARPS];
-    __shared__ int abort_flag;
+    __shared__ int abort_flag;  // a wait of this CTA has run out: it sends and requests nothing any more, and its part of every row to come is NaN
+    __shared__ uint32_t requested;       // copies
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = vf_rank(), size = gridDim.x;
     if (tid == 0) {
         abort_flag = 0;
+        requested = 0;
         tc_mbar_init(tc_smem(&bar), 1);
         tc_mbar_init(tc_smem(&xbar[0]), 1);
         tc_mbar_init(tc_smem(&xbar[1]), 1);
@@ -114,32 +145,27 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
     };
     auto bytes_ahead = [&](uint32_t lo, uint32_t hi) { return (hi - lo) / V * V * (uint32_t)sizeof(T); };
     auto request = [&](int row) {  // whole pieces of the slice
-        if (!AHEAD || tid != 0 || row >= a.rows) return;
+        if (!AHEAD || tid != 0 || row >= a.rows || abort_flag) return;  // (a copy given up on may still be open: the barrier and the memory stay its own)
         const uint32_t skip = skip_of(row);
         uint32_t lo, hi;
         range(skip, lo, hi);
         const uint32_t bytes = bytes_ahead(lo, hi);
         if (bytes == 0) return;
+        ++requested;
         tc_mbar_expect_tx(tc_smem(&bar), bytes);
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                      ::"r"(tc_smem(staged)), "l"(base + (size_t)row * a.stride_l - skip + lo), "r"(bytes), "r"(tc_smem(&bar)) : "memory");
     };
     request(blockIdx.y);
-    // Into everyone's slots, in turns.  A peer writes a turn's slots again only two rows on, and by then it has had this CTA's value of the row
-    // between, which is sent behind the last read of these.
-    uint32_t turn = 0, phase = 0, bar_phase = 0;
-    bool begun = false;
+    uint32_t bar_phase = 0;
+    RowExchange rows;
+    SoftmaxPort port{xchg, xbar, 0ull, &abort_flag, rank, size, tid};
     auto exchange = [&](unsigned long long v) {
-        if (!begun) vf_cluster_wait();
-        begun = true;
-        if (tid == 0) tc_mbar_expect_tx(tc_smem(&xbar[turn]), 8 * size);
-        if (tid < (int)size) vf_st_async(vf_peer(&xchg[turn][rank], (uint32_t)tid), v, vf_peer(&xbar[turn], (uint32_t)tid));
-        const bool ok = tc_mbar_wait(tc_smem(&xbar[turn]), phase, &abort_flag);
-        if (!ok) abort_flag = 1;
-        return ok;
+        port.value = v;
+        return rows.exchange(port);
     };
 
-    for (int row = blockIdx.y; row < a.rows; row += gridDim.y, phase ^= turn, turn ^= 1u) {
+    for (int row = blockIdx.y; row < a.rows; row += gridDim.y, rows.next_row()) {
         const uint32_t skip = skip_of(row);
         uint32_t lo, hi;
         range(skip, lo, hi);
@@ -149,7 +175,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
         const float inv_t = 1.f / t > 2.0e38f ? 2.0e38f * 1.442695041f : 1.442695041f / t;  // finite: (x - m) / T stays 0 where x = m, however small T
         bool here = true;
         if (AHEAD && bytes_ahead(lo, hi)) {
-            here = tc_mbar_wait(tc_smem(&bar), bar_phase, &abort_flag);
+            here = tc_mbar_try(tc_smem(&bar), bar_phase) || (!abort_flag && tc_mbar_wait(tc_smem(&bar), bar_phase, &abort_flag));  // (given up: whatever it is, the row is NaN)
             if (!here) abort_flag = 1;
             bar_phase ^= 1u;
         }
@@ -212,7 +238,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
             for (int w = 0; w < WARPS; ++w) best = best > part[w] ? best : part[w];
             here = exchange(best) && here;
             best = 0;
-            for (uint32_t c = 0; c < size; ++c) best = best > xchg[turn][c] ? best : xchg[turn][c];
+            for (uint32_t c = 0; c < size; ++c) best = best > xchg[rows.turn()][c] ? best : xchg[rows.turn()][c];
             // a row of -inf (and NaN) alone has no largest
             const uint32_t at = (uint32_t)(best >> 32) > 0x007fffffu ? (uint32_t)~(uint32_t)best : 0xffffffffu;
             for (uint32_t i = first; i < hi; i += STEP) {
@@ -284,7 +310,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
         if (!exchange(((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s))) s = nan;
         float top, sum;
         {  // a CTA's pair per lane
-            const unsigned long long v = xchg[turn][lane % VF_CLUSTER < size ? lane % VF_CLUSTER : 0];
+            const unsigned long long v = xchg[rows.turn()][lane % VF_CLUSTER < size ? lane % VF_CLUSTER : 0];
             const bool one = lane % VF_CLUSTER < size;
             const float mc = __uint_as_float((uint32_t)(v >> 32)), sc = __uint_as_float((uint32_t)v);
             top = mc;
@@ -294,7 +320,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
 #pragma unroll
             for (int o = VF_CLUSTER / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        const float inv = sum == 0.f ? 0.f : s != s ? s : 1.f / sum;  // (NaN among this CTA's values, or a peer that never came)
+        const float inv = s != s ? s : sum == 0.f ? 0.f : 1.f / sum;  // (NaN among this CTA's values, or a peer that never came)
         if constexpr (EPT > 0) {
             const float f = (m == -INFINITY ? 1.f : sm_exp(m, top, inv_t)) * inv;
 #pragma unroll
@@ -312,9 +338,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
             }
         }
     }
+    rows.leave(port);
     // A copy that a wait gave up on still writes to this memory: it has landed, or its time is long over.
     if constexpr (AHEAD)
-        if (abort_flag) tc_warp_drain(tc_smem(&bar), bar_phase ^ 1u);
+        if (abort_flag) tc_warp_drain(tc_smem(&bar), (requested - 1) & 1u);
 }
 
 // ------------------------------------------------------------------ verification of drafted tokens
