@@ -26,6 +26,8 @@
 #include "paged.cuh"
 #include "prefix_plan.hpp"
 
+#include <type_traits>
+
 namespace lcu {
 
 struct PrefixArgs {
@@ -296,7 +298,8 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         if (t == 0 || p.two) load_q(p);
         while (p.unit < sh->unit1) {
             const bool active = t == 0 || p.two, some = active && 128 * t + q * 32 < p.rows;  // ... of this warp's rows
-            float ref = -INFINITY, l = 0.f;
+            float top = -INFINITY, ref = -INFINITY, l = 0.f;  // the largest score; times scale2: what weights are relative to; their sum
+            bool far = true;                                  // of the warp: a ref is so large that its rounding counts, or there is none yet
             if (active) {
                 unsigned bad = bad_pages(p.j0);
                 for (int j = p.j0; j < p.j1; ++j, ++mine) {
@@ -330,11 +333,12 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                         for (int c = 0; c < 128; c += 8)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) m4[i] = at_max3(m4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
-                        const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale2;
-                        if (__any_sync(0xffffffffu, m > ref)) {
+                        const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), m = most * a.scale2;
+                        if (__any_sync(0xffffffffu, m > ref) || far) {
                             const float mn = fmaxf(ref, m), corr = ref == -INFINITY ? 0.f : at_exp2(ref - mn);
                             l *= corr;
                             ref = mn;
+                            top = fmaxf(top, most);
                             if (j > p.j0) {
 #pragma unroll 1
                                 for (int c = 0; c < DH; c += 16) {
@@ -346,28 +350,37 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                                     at_st16(to + c, o);
                                 }
                             }
+                            far = __any_sync(0xffffffffu, fabsf(ref) >= 4096.f);
                         }
-                        const float sub = ref == -INFINITY ? 0.f : ref;  // a row whose scores are all -inf keeps zero weights
-                        const unsigned long long mul = at_pair(a.scale2, a.scale2), off = at_pair(-sub, -sub);
+                        const unsigned long long mul = at_pair(a.scale2, a.scale2);
                         unsigned long long l2[2] = {0ull, 0ull};
+                        auto weights = [&](auto difference_first, float sub) {
+                            const unsigned long long off = at_pair(-sub, -sub);
 #pragma unroll
-                        for (int h = 0; h < 8; ++h) {
-                            uint32_t w[8];
+                            for (int h = 0; h < 8; ++h) {
+                                uint32_t w[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int c = 16 * h + 2 * i;
-                                const float2 x = at_unpair(at_fma2(at_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul, off));
-                                const float y0 = at_exp2(x.x), y1 = at_exp2(x.y);
-                                w[i] = Act<T>::pack(y0, y1);
-                                l2[i & 1] = at_add2(l2[i & 1], at_pair(y0, y1));
+                                for (int i = 0; i < 8; ++i) {
+                                    const int c = 16 * h + 2 * i;
+                                    const unsigned long long v = at_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                                    const float2 x = at_unpair(difference_first ? at_fma2(at_add2(v, off), mul, 0ull) : at_fma2(v, mul, off));
+                                    const float y0 = at_exp2(x.x), y1 = at_exp2(x.y);
+                                    w[i] = Act<T>::pack(y0, y1);
+                                    l2[i & 1] = at_add2(l2[i & 1], at_pair(y0, y1));
+                                }
+                                pf_st8(ts + 8 * h, w);
+                                if (h == 3) {
+                                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                    pf_arrive(pr, lane);
+                                }
                             }
-                            pf_st8(ts + 8 * h, w);
-                            if (h == 3) {
-                                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                                pf_arrive(pr, lane);
-                            }
-                        }
+                        };
+                        // ref is rounded and the product inside the FMA is not: a row's weights are all off by the same factor, 2^(half a step of ref).
+                        // Steps of 2^-12 and less are nothing; beyond, the difference to the largest score comes first, so that weights end at 1.
+                        // (Two copies cost 1 %; one, with scores that a branch may have changed, 3 to 4.)
+                        if (far) weights(std::true_type{}, top == -INFINITY ? 0.f : top);  // (a row whose scores are all -inf keeps zero weights)
+                        else weights(std::false_type{}, ref);
                         const float2 la = at_unpair(at_add2(l2[0], l2[1]));
                         l += la.x + la.y;
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
