@@ -21,7 +21,9 @@
 //
 // f32 scores and softmax, sums in f32 over the weights as they are, weights rounded to the activation type ahead of the second product (its
 // operands are 16-bit), one rounding of the output.  (Sums over the rounded weights, as attention.cu takes them, are no closer to the
-// softmax where many weights count and cost 4 % of the prefix in conversions; a weight that stands alone is 1 and is not rounded.)
+// softmax where many weights count and cost 4 % of the prefix in conversions; a weight that stands alone is a power of two and is not rounded.)
+// The largest weight of a part is 1, but 2^14 in f16: f16 ends at 2^-24, and below a 1 thousands of keys 2^-25 of it each would be in the sum and
+// not in the product.  The power of two is in the maximum that a part is relative to, so the sum of parts knows nothing of it.
 #include "attention_tc.cuh"
 #include "paged.cuh"
 #include "prefix_plan.hpp"
@@ -29,6 +31,14 @@
 #include <type_traits>
 
 namespace lcu {
+
+template <class T> constexpr float PF_TOP = 0.f;  // the largest weight is 2^PF_TOP
+template <> constexpr float PF_TOP<__half> = 14.f;
+// what weights are relative to, of the largest scaled score (rounded up: no weight is above the largest, however large the scores)
+template <class T> __device__ __forceinline__ float pf_reference(float n) {
+    if constexpr (PF_TOP<T> != 0.f) return __fsub_ru(n, PF_TOP<T>);
+    return n;
+}
 
 struct PrefixArgs {
     void *o;
@@ -298,7 +308,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
         if (t == 0 || p.two) load_q(p);
         while (p.unit < sh->unit1) {
             const bool active = t == 0 || p.two, some = active && 128 * t + q * 32 < p.rows;  // ... of this warp's rows
-            float top = -INFINITY, ref = -INFINITY, l = 0.f;  // the largest score; times scale2: what weights are relative to; their sum
+            float top = -INFINITY, ref = -INFINITY, l = 0.f;  // the largest score; what weights are relative to; their sum
             bool far = true;                                  // of the warp: a ref is so large that its rounding counts, or there is none yet
             if (active) {
                 unsigned bad = bad_pages(p.j0);
@@ -333,7 +343,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                         for (int c = 0; c < 128; c += 8)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) m4[i] = at_max3(m4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
-                        const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), m = most * a.scale2;
+                        const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), m = pf_reference<T>(most * a.scale2);
                         if (__any_sync(0xffffffffu, m > ref) || far) {
                             const float mn = fmaxf(ref, m), corr = ref == -INFINITY ? 0.f : at_exp2(ref - mn);
                             l *= corr;
@@ -354,8 +364,8 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                         }
                         const unsigned long long mul = at_pair(a.scale2, a.scale2);
                         unsigned long long l2[2] = {0ull, 0ull};
-                        auto weights = [&](auto difference_first, float sub) {
-                            const unsigned long long off = at_pair(-sub, -sub);
+                        auto weights = [&](auto difference_first, float sub, float plus) {
+                            const unsigned long long off = at_pair(-sub, -sub), off2 = at_pair(plus, plus);
 #pragma unroll
                             for (int h = 0; h < 8; ++h) {
                                 uint32_t w[8];
@@ -363,7 +373,7 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                                 for (int i = 0; i < 8; ++i) {
                                     const int c = 16 * h + 2 * i;
                                     const unsigned long long v = at_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                                    const float2 x = at_unpair(difference_first ? at_fma2(at_add2(v, off), mul, 0ull) : at_fma2(v, mul, off));
+                                    const float2 x = at_unpair(difference_first ? at_fma2(at_add2(v, off), mul, off2) : at_fma2(v, mul, off));
                                     const float y0 = at_exp2(x.x), y1 = at_exp2(x.y);
                                     w[i] = Act<T>::pack(y0, y1);
                                     l2[i & 1] = at_add2(l2[i & 1], at_pair(y0, y1));
@@ -377,10 +387,12 @@ prefix_tc_kernel(const PrefixArgs a, const __grid_constant__ CUtensorMap map_k, 
                             }
                         };
                         // ref is rounded and the product inside the FMA is not: a row's weights are all off by the same factor, 2^(half a step of ref).
-                        // Steps of 2^-12 and less are nothing; beyond, the difference to the largest score comes first, so that weights end at 1.
+                        // Steps of 2^-12 and less are nothing; beyond, the difference to the largest score comes first, so that weights end where they should.
                         // (Two copies cost 1 %; one, with scores that a branch may have changed, 3 to 4.)
-                        if (far) weights(std::true_type{}, top == -INFINITY ? 0.f : top);  // (a row whose scores are all -inf keeps zero weights)
-                        else weights(std::false_type{}, ref);
+                        if (far) {
+                            const bool none = top == -INFINITY;  // a row whose scores are all -inf keeps zero weights
+                            weights(std::true_type{}, none ? 0.f : top, none ? 0.f : __fmul_rn(top, a.scale2) - ref);
+                        } else weights(std::false_type{}, ref, 0.f);
                         const float2 la = at_unpair(at_add2(l2[0], l2[1]));
                         l += la.x + la.y;
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -668,8 +680,8 @@ __global__ void __launch_bounds__(OW_THREADS, DEPTH == 1 ? 8 : 5) own_kernel(con
                 s[h][e] = seen && key < see0 ? s[h][e] * a.scale2 : -INFINITY;
                 s[h][2 + e] = seen && key < see1 ? s[h][2 + e] * a.scale2 : -INFINITY;
             }
-        const float n0 = fmaxf(m0, ow_quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]))));
-        const float n1 = fmaxf(m1, ow_quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]))));
+        const float n0 = fmaxf(m0, pf_reference<T>(ow_quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])))));
+        const float n1 = fmaxf(m1, pf_reference<T>(ow_quad_max(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])))));
         const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
         const float f0 = m0 == -INFINITY ? 1.f : at_exp2(m0 - b0), f1 = m1 == -INFINITY ? 1.f : at_exp2(m1 - b1);  // (a row that has seen nothing has nothing to scale)
         m0 = n0;

@@ -1,4 +1,5 @@
 """Weights of the attention of a shared prefix at the ends of their range (needs a B200)."""
+import numpy as np
 import pytest
 import torch
 
@@ -47,3 +48,28 @@ def test_scores_of_billions(L, dt, tokens, nh, nkvh, dh, prefix, own, scale):
         off = (b.o[t].double() - want).abs()
         tol = HALF[dt] * want.abs() + ((prefix + own) / 16 + 64) * 2.0 ** -23 * mag + 2.0 ** -24
         assert b.o[t].isfinite().all() and (off <= tol).all(), f"token {t}: {float(off.max())} off, {float((off / tol).max())} of what is allowed"
+
+
+@pytest.mark.parametrize("dt", [0, 1])
+@pytest.mark.parametrize("tokens,nh,nkvh,dh,prefix,own", SHAPES)
+@pytest.mark.parametrize("below", [25.1, 27.5])
+def test_many_keys_far_below_one(L, dt, tokens, nh, nkvh, dh, prefix, own, below):
+    """The first key of all outweighs each of the others 2^25.1 and 2^27.5 times, but these are thousands, and their values are all the result there
+    is.  A weight may be off by half a step of its type, as in any batch."""
+    page = 64
+    b = Batch(tokens + prefix, [(own, 1)] * tokens, prefix, nh, nkvh, dh, dt, page)
+    sink, flat = (int(p) for p in (b.prefix_ids if prefix else b.ids[0])[:2])
+    b.prefix_ids[1:] = flat
+    b.ids[:] = flat
+    if not prefix:
+        b.ids[:, 0] = sink
+    b.pool.zero_()
+    b.pool[:, 1] = 512.0
+    b.pool[sink, 1, :, 0] = 0.0
+    b.q.zero_()
+    b.q[..., 5] = 8.0
+    b.scale = 0.125
+    b.pool[sink, 0, :, 0, 5] = below * float(np.log(2.0))  # (rounded to the type: the check reads what is there)
+    b.run(L)
+    only(b, list(range(0, tokens, 97)))
+    b.check()
