@@ -521,7 +521,7 @@ LCU_API int lcu_argmax_rows_noalloc(lcu_kv_pair *out, const void *logits, int ro
 typedef struct {
     void *k, *v;
     int64_t stride_page;  /* elements */
-    int32_t stride_tok, stride_head;
+    int32_t stride_tok, stride_head;  /* stride_head is not read where there is one KV head */
     int32_t n_pages;      /* ids outside [0, n_pages) name no page */
     int32_t page_tokens;  /* power of two in [8,128] */
 } lcu_kv_pages;

@@ -529,11 +529,13 @@ static int rows_run(RowsArgs &a, const lcu_qk_prep *prep, int n, int dt, const c
     return rows_t<float>(a, n, vec, s);
 }
 
-int kv_pages_check(const lcu_kv_pages *p, const char *who) {
+int kv_pages_take(lcu_kv_pages *out, const lcu_kv_pages *p, int nkvh, const char *who) {
     LCU_REQUIRE(p && p->k && p->v && p->n_pages >= 1, "%s: no pages", who);
     LCU_REQUIRE(p->page_tokens >= 8 && p->page_tokens <= 128 && (p->page_tokens & (p->page_tokens - 1)) == 0,
                 "%s: pages of %d tokens (a power of two in [8,128])", who, p->page_tokens);
-    LCU_REQUIRE(p->stride_page > 0 && p->stride_tok > 0 && p->stride_head >= 0, "%s: page strides", who);
+    LCU_REQUIRE(p->stride_page > 0 && p->stride_tok > 0 && (nkvh <= 1 || p->stride_head > 0), "%s: page strides", who);
+    *out = *p;
+    if (nkvh == 1) out->stride_head = out->stride_tok;
     return LCU_OK;
 }
 
@@ -554,15 +556,15 @@ extern "C" int lcu_op_qk_norm_rope(void *q_out, int stqo, int shqo, const void *
 extern "C" int lcu_op_kv_append(const lcu_kv_pages *pages, const int32_t *table, int table_stride, int n_seq, const int32_t *tok_seq, const uint32_t *slot,
                                 const void *k, int stk, int shk, const void *v, int stv, int shv, void *q_out, int stqo, int shqo, const void *q, int stq,
                                 int shq, const uint32_t *pos, const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s) {
-    int rc = kv_pages_check(pages, "kv_append");
+    RowsArgs a{};
+    int rc = kv_pages_take(&a.pages, pages, nkvh, "kv_append");
     if (rc) return rc;
     LCU_REQUIRE(n <= 0 || (table && tok_seq && slot && k && v && (nh <= 0 || (q && q_out))), "kv_append: null argument");
     LCU_REQUIRE(table_stride >= 1 && n_seq >= 1 && nkvh >= 1, "kv_append: %d sequences of %d pages, %d KV heads", n_seq, table_stride, nkvh);
     LCU_REQUIRE(nh == 0 || prep, "kv_append: queries without what to do with them");
-    RowsArgs a{};
     a.q = q; a.stq = stq; a.shq = shq; a.q_out = q_out; a.stqo = stqo; a.shqo = shqo;
     a.k = k; a.stk = stk; a.shk = shk; a.v = v; a.stv = stv; a.shv = shv;
-    a.pages = *pages; a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.slot = slot;
+    a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.slot = slot;
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
     a.pos = pos; a.nh = nh; a.nkvh = nkvh; a.n_v = nkvh; a.dh = dh;
     return rows_run(a, prep, n, dt, "kv_append", as_stream(s));

@@ -22,6 +22,7 @@ class OncePerDevice {
     }
 };
 
-int kv_pages_check(const lcu_kv_pages *p, const char *who);
+// checks a caller's pages, and copies them with a stride from head to head that may be used where there is one KV head (whose stride nobody reads)
+int kv_pages_take(lcu_kv_pages *out, const lcu_kv_pages *p, int nkvh, const char *who);
 
 }  // namespace lcu

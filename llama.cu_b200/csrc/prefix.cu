@@ -922,7 +922,8 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
                                        uint32_t prefix_len, const int32_t *table, int table_stride, int n_seq, const int32_t *tok_seq,
                                        const uint32_t *tok_ctx, int n, int nh, int nkvh, int dh, float scale, int dt, void *workspace,
                                        size_t workspace_len, lcu_stream_t s) {
-    int rc = kv_pages_check(pages, "attention_prefix");
+    PrefixArgs a{};
+    int rc = kv_pages_take(&a.pages, pages, nkvh, "attention_prefix");
     if (rc) return rc;
     LCU_REQUIRE(dt == LCU_F16 || dt == LCU_BF16, "attention_prefix: dtype %d unsupported", dt);
     LCU_REQUIRE(dh == 64 || dh == 128, "attention_prefix: dh = %d unsupported (64, 128)", dh);
@@ -935,14 +936,13 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     LCU_REQUIRE(!prefix_len || prefix_fits(n, nh / nkvh, nkvh, prefix_len), "attention_prefix: prefix of %u for %d tokens of %d heads: more than a call takes", prefix_len, n, nh);
     LCU_REQUIRE(o && q && tok_seq && tok_ctx && (prefix_table || !prefix_len) && (table || !table_stride), "attention_prefix: null argument");
     LCU_REQUIRE((((uintptr_t)o | (uintptr_t)q | (uintptr_t)pages->k | (uintptr_t)pages->v) % 16) == 0 && (sto | sho | stq | shq) % 8 == 0 &&
-                    pages->stride_page % 8 == 0 && pages->stride_tok % 8 == 0 && pages->stride_head % 8 == 0 && pages->stride_head > 0,
+                    pages->stride_page % 8 == 0 && pages->stride_tok % 8 == 0 && a.pages.stride_head % 8 == 0,
                 "attention_prefix: rows of q, o and the pages start on 16 bytes");
     const size_t need = lcu_attention_prefix_workspace_size(n, nh, nkvh, dh, prefix_len);
     LCU_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0 && workspace_len >= need), "attention_prefix: workspace of %zu bytes, %zu needed (256-byte aligned)",
                 workspace_len, need);
-    PrefixArgs a{};
     a.o = o; a.sto = sto; a.sho = sho; a.q = q; a.stq = stq; a.shq = shq;
-    a.pages = *pages; a.prefix_table = prefix_table; a.prefix_len = prefix_len;
+    a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.tok_ctx = tok_ctx;
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
     a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale * 1.4426950408889634f;
