@@ -558,7 +558,7 @@ LCU_API int lcu_op_kv_append(const lcu_kv_pages *pages, const int32_t *table, in
                              const lcu_qk_prep *prep, int n, int nh, int nkvh, int dh, int dt, lcu_stream_t s);
 /* Attention of n tokens whose sequences begin with the same prefix: token t sees the first prefix_len slots of the pages prefix_table and
  * the first tok_ctx[t] slots of its sequence's own pages (table, as above; positions of the prefix are not repeated there).  o, q
- * [n, nh, dh]; query head h reads KV head h / (nh / nkvh); scores are scaled by `scale` > 0.  dh 64 or 128, nh / nkvh up to 16, dt LCU_F16 or LCU_BF16.
+ * [n, nh, dh]; query head h reads KV head h / (nh / nkvh); scores are scaled by `scale`, in (0, 2.3e38).  dh 64 or 128, nh / nkvh up to 16, dt LCU_F16 or LCU_BF16.
  * ceil(n nh / nkvh / 256) nkvh ceil(prefix_len / 128) up to 2^28.  The prefix is read once for all tokens (a short one of few tokens once each).  f32 scores and softmax, weights rounded to dt ahead of the product with the values (f16: those
  * below 2^-28 of the largest to multiples of 2^-38 of it), one rounding of the output.  Rows of q, o and the pages start on 16 bytes.  Tokens with tok_seq outside [0, n_seq) are left unwritten; tok_ctx counts at
  * most table_stride pages; positions on page ids that name no page are not seen; a token that sees nothing gets zeros.  (Waits inside the

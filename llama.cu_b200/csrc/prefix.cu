@@ -929,7 +929,8 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     LCU_REQUIRE(dh == 64 || dh == 128, "attention_prefix: dh = %d unsupported (64, 128)", dh);
     LCU_REQUIRE(n >= 0 && n <= 65535 && nkvh >= 1 && nkvh <= 65535 && nh >= nkvh && nh % nkvh == 0 && nh / nkvh <= 16,
                 "attention_prefix: %d tokens, %d query heads over %d", n, nh, nkvh);
-    LCU_REQUIRE(scale > 0.f && scale < INFINITY, "attention_prefix: scale %g", (double)scale);
+    const float scale2 = scale * 1.4426950408889634f;  // finite too: a score of 0 stays one
+    LCU_REQUIRE(scale > 0.f && scale2 < INFINITY, "attention_prefix: scale %g", (double)scale);
     LCU_REQUIRE(prefix_len <= 0x7fffffffu && table_stride >= 0 && (long long)table_stride * pages->page_tokens <= 0x7fffffffll && n_seq >= 1,
                 "attention_prefix: prefix of %u, %d sequences of %d pages", prefix_len, n_seq, table_stride);
     if (n == 0) return LCU_OK;
@@ -945,7 +946,7 @@ extern "C" int lcu_op_attention_prefix(void *o, int sto, int sho, const void *q,
     a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.table = table; a.table_stride = table_stride; a.n_seq = n_seq; a.tok_seq = tok_seq; a.tok_ctx = tok_ctx;
     while ((1 << a.page_shift) < pages->page_tokens) ++a.page_shift;
-    a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale * 1.4426950408889634f;
+    a.n = n; a.nh = nh; a.nkvh = nkvh; a.scale2 = scale2;
     if (prefix_len && prefix_walk(n, nh / nkvh, nkvh, prefix_len, (long long)table_stride * pages->page_tokens, sm_count(), dh)) {
         a.walk_len = prefix_len;
         a.prefix_len = 0;
