@@ -573,6 +573,8 @@ LCU_API int lcu_op_attention_prefix(void *o, int stride_tok_o, int stride_head_o
 /* probs[r, j] = exp((x_j - max) / T) / sum over the n logits of row r, f32; T = temperature[r] (device, finite, >= 0; NULL: 1 everywhere).  T = 0: 1 at
  * the lowest index of the largest logit, 0 elsewhere.  Logits of dtype dt (F16, BF16, F32); strides from row to row in elements.
  * Logits of -inf get 0; a row of nothing else gets zeros; with T > 0 a row that holds NaN or +inf is NaN, with T = 0 NaN never is the largest.
+ * (What lcu_step samples from, on logits in the activation dtype, where its lcu_sample_args say no more than a temperature: top_p 1, top_k the vocabulary
+ * or more.  A smaller top_p or top_k has no counterpart here, and tokens drafted with one were drawn from other probabilities than these.)
  * probs may be the logits (F32, same stride), and may not overlap them otherwise.  (Waits inside the kernel are bounded: values that one which ran out
  * left without their row's maximum and sum are NaN.) */
 LCU_API int lcu_op_softmax_rows(float *probs, size_t stride_p, const void *logits, size_t stride_l, const float *temperature, int rows, size_t n, int dt,

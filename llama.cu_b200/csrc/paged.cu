@@ -4,15 +4,15 @@
 //   y = x w / sqrt(mean(x^2) + eps)                   per head, where there are weights
 //   (a, b) -> (a cos - b sin, a sin + b cos)          of the first rot_dims values, pairs (2 i, 2 i + 1) or (i, i + rot_dims / 2)
 //
-// all in 32 bits with one rounding at the end.  Every row is read once and written once, so HBM is the floor; what has to be kept down
-// on the way there is instructions and waits.  heads_kernel: a row is held by dh / 16 lanes, each with 8 values of the lower half and the
+// all in 32 bits with one rounding at the end.  Every row is read once and written once, so HBM is the floor; the bound is instructions: 61 to 65 % of
+// the issue slots are taken at a prompt's sizes, with the four warps to a scheduler that the registers leave, and memory is at 40 % and less.  heads_kernel: a row is held by dh / 16 lanes, each with 8 values of the lower half and the
 // 8 that stand dh / 2 behind them, so that the pairs of either kind meet in one thread; lanes stay with their head from token to token
 // and request the next token's row while they work on one.  rows_kernel takes heads of an
 // odd number of pieces (dh 72, 40, ..), rows_any_kernel the rest (sizes, strides or addresses that are no multiples of 16 bytes).
 //
-// Measured on a B200: 8000 tokens of 32 + 8 heads of 64 (bf16, pairs side by side, 83 MB) 22.6 us, 3.7 TB/s, where adding a number to as many
-// values takes 16.2; 8004 tokens of 32 + 8 + 8 heads of 128 with norms into pages (halves, 201 MB) 43.7 us, 4.6 TB/s of 32.8; one token 5 us, which
-// is launch and three round trips.
+// Measured on a B200 (calls in a graph, per call): 8000 tokens of 32 + 8 heads of 64 with norms (f16, pairs side by side, half of a head turned, 83 MB)
+// 21.1 us, 3.9 TB/s, where adding a number to as many values takes 16.2, and 42.5 in f32 (165 MB); 8004 tokens of 32 + 8 + 8 heads of 128 with norms into
+// pages (bf16, halves, 201 MB) 42.4 us, 4.7 TB/s, of 32.8, and 97.9 in f32 (398 MB); one token 2.0, 33 tokens into pages 2.2.
 #include "paged.cuh"
 
 #include <mutex>
@@ -21,7 +21,7 @@ namespace lcu {
 
 constexpr int RW_THREADS = 256;
 constexpr int RW_MAX_HEAD = 256;
-constexpr int HK_THREADS = 128, HK_STAGES = 4, HK_BLOCKS = 5;  // (4 blocks of 16-bit rows on an SM 3 % slower, 6 spill registers and are a third slower)
+constexpr int HK_THREADS = 128, HK_STAGES = 4, HK_BLOCKS = 5;  // (4 blocks of 16-bit rows on an SM 3 % slower, 6 a third; with 5, 24 of the 48 forms spill one or two registers)
 
 struct RowsArgs {
     const void *q, *k, *v;
@@ -147,7 +147,7 @@ __device__ __forceinline__ unsigned long long rw_mul2(unsigned long long x, unsi
 enum { SIDE_BY_SIDE, HALVES_WHOLE, HALVES_PART };
 
 // LPR lanes hold a row of dh <= 16 LPR values, each 8 from d on and 8 from d + gap on: gap is dh / 2 or, in HALVES_PART, half of the rotated part or half
-// of the rest (46.7 us where HALVES_WHOLE has 43.7).  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every
+// of the rest (8004 tokens whose halves are whole heads: 46.7 us where HALVES_WHOLE has 43.7, host included).  WF: the norms' weights are f32.  blockDim.x / LPR rows from blockIdx.y's first on, every
 // gridDim.x-th token.
 template <class T, int LPR, int MODE, bool WF>
 __global__ void __launch_bounds__(HK_THREADS, sizeof(T) == 2 ? HK_BLOCKS : 4) heads_kernel(const RowsArgs a, int n, int rows_per) {
@@ -470,8 +470,8 @@ static int rows_t(const RowsArgs &a, int n, bool vec, cudaStream_t s) {
         LCU_CHECK_CUDA(cudaGetLastError());
         return LCU_OK;
     }
-    // (Halves are in pieces of 8 where rot is a multiple of 16, which `vec` says.)  4000 tokens of 32 + 8 + 8 heads of 128 with norms, rot 64 by halves: 25.9
-    // us here, 35 in rows_kernel; heads of 80 with rot 40 by halves, whose pieces begin off 16 bytes, 82 in rows_any_kernel.
+    // (Halves are in pieces of 8 where rot is a multiple of 16, which `vec` says.)  4000 tokens of 32 + 8 + 8 heads of 128 with norms, rot 64 by halves: 24.4
+    // us here, 35 in rows_kernel; heads of 80 with rot 40 by halves, whose pieces begin off 16 bytes, 79.6 in rows_any_kernel.
     if (a.dh % 16 == 0) {
         const int lanes = a.dh / 16;
         return lanes <= 2 ? heads_form<T, 2>(a, n, s) : lanes <= 4 ? heads_form<T, 4>(a, n, s) : lanes <= 8 ? heads_form<T, 8>(a, n, s) : heads_form<T, 16>(a, n, s);

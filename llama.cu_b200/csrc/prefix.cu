@@ -15,9 +15,10 @@
 //  - The sum of all parts: at the end of own_kernel where its blocks, their rows and the parts are few, else in own_sum_kernel.
 //  - A prefix that is short next to the number of tokens is read by own_kernel too, ahead of the token's own slots, and the call is one launch.
 //
-// Measured on a B200, heads of 128: 256 tokens of 64 heads over 8 behind 32000 positions 284 us (0.95 PFLOP/s; exponentials and products take
-// turns) and 341 in long runs at 1000 W; 16 x 5 drafted tokens of 32 over 8 behind 8001 35 us: prefix 22 (15 of units, 7 to begin, end and leave
-// parts), own slots 9, sum 4.
+// Measured on a B200 (calls in a graph), heads of 128: 256 tokens of 64 heads over 8 behind 32000 positions 293 us (0.92 PFLOP/s; exponentials and products
+// take turns, half of the time each) and 324 in long runs at 1000 W; 16 x 5 drafted tokens of 32 over 8 behind 8001 35.4 us: prefix 22 (15 of units, 7 to
+// begin, end and leave parts), own slots 9, sum 4.  A unit there is a chain: scores, maximum, accumulator, exponentials, products, one warp to a scheduler
+// and tile; tensor cores, exponentials and issue slots are each busy a quarter of the time.
 //
 // f32 scores and softmax, sums in f32 over the weights as they are, weights rounded to the activation type ahead of the second product (its
 // operands are 16-bit), one rounding of the output.  (Sums over the rounded weights, as attention.cu takes them, are no closer to the

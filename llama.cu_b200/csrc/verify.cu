@@ -350,11 +350,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) softmax_kernel(const SoftmaxArg
 //   behind the accepted ones comes the first index whose running sum of w exceeds u_last sum(w):
 //   w = max(p - q, 0) at the rejected draft (p itself where nothing is left), w = p behind the last draft
 //
-// in 64 bits, where the products u q and the differences of 32-bit numbers are exact.  Bound by HBM: of all rows only the pair that the last token is drawn
-// from is read whole.  A cluster of up to 8 CTAs takes a sequence: sums of pieces of 512 values or more, totals across the cluster
-// in one exchange, and the CTA that the threshold falls into reads the one piece that holds it again.  The order of the sums is fixed.
-// Measured on a B200, f32: 64 sequences of 128256 tokens 21 us (66 MB; a plain sum of 82 MB takes 22.3), 30 where rows begin off 16 bytes; one sequence of
-// 32000 6.5, a chain of drafts, gathers, row, cluster and piece.
+// Products u q and comparisons are exact (in 64 bits, of 32-bit numbers); differences and sums are rounded to 2^-53, the total and the scan that finds the
+// token each in a fixed order of their own, so a threshold that close to a running sum falls to either side.  Bound by HBM: of all rows only the pair
+// that the last token is drawn from is read whole.  A cluster of up to 8 CTAs takes a sequence: sums of pieces of 512 values or more, totals across the cluster
+// in one exchange, and the CTA that the threshold falls into reads the one piece that holds it again.
+// Measured on a B200 (calls in a graph), f32: 64 sequences of 128256 tokens 21.1 us (66 MB at most, a row less for each sequence that accepts all; a plain
+// sum of 82 MB takes 22.3), 27.8 of 128257, whose rows begin off 16 bytes; bf16 19.9; one sequence of 32000 6.3, a chain of drafts, gathers, row, cluster and
+// piece.
 struct VerifyArgs {
     int32_t *accepted, *tokens;
     const void *target, *draft;
